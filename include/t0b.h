@@ -37,6 +37,9 @@ enum {
 
 /* ggml tensor type ids (gguf.rs:32-39) */
 enum { T0B_F32 = 0, T0B_F16 = 1, T0B_Q4_0 = 2, T0B_Q8_0 = 8 };
+/* element type of the 4-bit operators' plain tensors beside F32 and F16 (the
+ * ggml type id of bfloat16) */
+enum { T0B_BF16 = 30 };
 
 typedef struct t0b_engine t0b_engine;
 typedef struct t0b_model t0b_model;
@@ -189,6 +192,89 @@ t0b_status t0b_qmatrix_swiglu(t0b_qmatrix *q0, t0b_qmatrix *q2, const float *x_d
                               const float *b2_dev, float *z_dev, float *y_dev, void *stream);
 /* Wait for `stream` and report any kernel-side error of q's launches. */
 t0b_status t0b_qmatrix_sync(t0b_qmatrix *q, void *stream);
+
+/* ---- 4-bit microscaled operators (no reference counterpart) ----
+ * Quantisation, expansion, product, gated product and MLP on matrices of
+ * 4-bit floats with one 8-bit scale per block of consecutive values of a row
+ * (device pointers; weights AND activations are 4-bit, multiplied by the
+ * block-scaled tensor-core instructions, sums in f32).
+ *
+ * A value is sign * {0, 0.5, 1, 1.5, 2, 3, 4, 6} * block scale * tensor_scale:
+ *   T0B_FP4_MX  blocks of 32, scale = 2^(byte - 127), byte 255 = NaN;
+ *               tensor_scale must be 1
+ *   T0B_FP4_NV  blocks of 16, scale = an unsigned float with 4 exponent (bias
+ *               7) and 3 mantissa bits, byte 127 = NaN; tensor_scale is any
+ *               positive normal number (a power of two in [2^-64, 2^64] where
+ *               a call quantises, so that every rounding is decided exactly)
+ *
+ * Layout of a matrix [rows, k] (any rows, k >= 1; k <= 2^20, rows < 2^30):
+ *   codes   row r starts at byte r * 16 * ceil(k / 32); value i is the low
+ *           (even i) or high (odd i) half of byte i / 2: sign bit and index.
+ *           Codes behind k are zero.  t0b_fp4_code_bytes bytes.
+ *   scales  tiles of 128 rows by 4 blocks: the byte of row r, block b is at
+ *           (r % 32) * 16 + (r % 128 / 32) * 4 + b % 4 of the 512-byte tile
+ *           (r / 128) * ceil(blocks / 4) + b / 4.  Bytes of rows and blocks
+ *           behind the matrix are zero.  t0b_fp4_scale_bytes bytes.
+ * Both arrays are 16-byte aligned.  The calls that write a matrix write all
+ * of both arrays, the zeros behind the matrix included.
+ *
+ * All calls only queue work on `stream` (cudaStream_t, NULL = legacy default
+ * stream) of the engine's device, allocate nothing, share no scratch between
+ * calls, leave the calling thread's current device as it was, and may be
+ * captured in CUDA graphs; calls on different streams and host threads may
+ * overlap.  Outputs must not overlap inputs.  Kernel-side errors (a bounded
+ * wait that ran out) are reported by t0b_fp4_sync.  Results do not depend on
+ * the stream, on the capture or on what else runs. */
+enum { T0B_FP4_MX = 1, T0B_FP4_NV = 2 };
+typedef struct {
+  int32_t format; /* T0B_FP4_MX or T0B_FP4_NV */
+  int32_t rows, k;
+  float tensor_scale;
+  uint8_t *codes;  /* device */
+  uint8_t *scales; /* device */
+} t0b_fp4;
+/* Sizes of a matrix's arrays (0 for an invalid shape or format). */
+size_t t0b_fp4_code_bytes(int rows, int k);
+size_t t0b_fp4_scale_bytes(int format, int rows, int k);
+
+/* x [out->rows, out->k] of x_type (T0B_F32, T0B_F16, T0B_BF16), row r at
+ * r * ldx elements, to 4 bits.  A block's scale is, with amax its largest
+ * magnitude: MX the largest power of two <= amax / 4 (not below 2^-127), NV
+ * amax / (6 tensor_scale) rounded to the nearest scale (ties to even, at most
+ * 448).  Values are x / scale rounded to nearest (ties to the even index), at
+ * most 6 in magnitude.  A block that holds a NaN or an infinity becomes NaN
+ * as a whole; a block whose scale rounds to zero becomes zero. */
+t0b_status t0b_fp4_quantize(t0b_engine *e, int x_type, const void *x_dev, int64_t ldx, const t0b_fp4 *out,
+                            void *stream);
+/* The values of `in`, rounded to y_type: y [in->rows, in->k], row r at r * ldy
+ * elements. */
+t0b_status t0b_fp4_dequantize(t0b_engine *e, const t0b_fp4 *in, int y_type, void *y_dev, int64_t ldy, void *stream);
+/* y [x->rows, w->rows] = x . w^T (+ bias[w->rows], f32, may be NULL), of
+ * y_type, row r at r * ldy elements; x and w of one format and k. */
+t0b_status t0b_fp4_gemm(t0b_engine *e, const t0b_fp4 *w, const t0b_fp4 *x, const float *bias_dev, int y_type,
+                        void *y_dev, int64_t ldy, void *stream);
+/* z = silu(x . gate^T + bg) * (x . up^T + bu), [x->rows, F] with w = gate rows
+ * [0, F), up rows [F, 2F) as t0b_swiglu_q's w0, bias [2F] or NULL.  Either
+ * z_dev (of z_type, row r at r * ldz elements) or zq (quantised as by
+ * t0b_fp4_quantize, of w's format, rows x->rows, k F) is given, the other
+ * NULL. */
+t0b_status t0b_fp4_glu(t0b_engine *e, const t0b_fp4 *w, const t0b_fp4 *x, const float *bias_dev, int z_type,
+                       void *z_dev, int64_t ldz, const t0b_fp4 *zq, void *stream);
+/* t0b_fp4_quantize + t0b_fp4_gemm in one call: x [xq->rows, xq->k] of x_type.
+ * xq gives the activations' format, shape and scale and the memory for their
+ * 4-bit form; what that memory holds afterwards is unspecified. */
+t0b_status t0b_fp4_linear(t0b_engine *e, const t0b_fp4 *w, int x_type, const void *x_dev, int64_t ldx,
+                          const t0b_fp4 *xq, const float *bias_dev, int y_type, void *y_dev, int64_t ldy,
+                          void *stream);
+/* The whole gated MLP: y = q(silu(q(x) . gate^T + bg) * (q(x) . up^T + bu)) . w2^T
+ * + b2, with q() the quantisations into xq [M, K] and zq [M, F] (their contents
+ * afterwards are unspecified); w0 [2F, K], w2 [N2, F], y [M, N2]. */
+t0b_status t0b_fp4_mlp(t0b_engine *e, const t0b_fp4 *w0, const t0b_fp4 *w2, int x_type, const void *x_dev, int64_t ldx,
+                       const t0b_fp4 *xq, const t0b_fp4 *zq, const float *b0_dev, const float *b2_dev, int y_type,
+                       void *y_dev, int64_t ldy, void *stream);
+/* Wait for `stream` and report any kernel-side error of the engine's 4-bit
+ * operators since the last call. */
+t0b_status t0b_fp4_sync(t0b_engine *e, void *stream);
 
 /* ---- bounded-wait self-test (no reference counterpart; a diagnostic) ----
  * Every wait of a kernel on an mbarrier (TMA tiles, dequantized tiles,

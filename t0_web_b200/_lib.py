@@ -13,6 +13,8 @@ LIB_PATH = os.path.join(_HERE, "libt0b.so")
 
 T0B_OK, T0B_ERR_INVALID, T0B_ERR_FORMAT, T0B_ERR_UNSUPPORTED, T0B_ERR_CUDA, T0B_ERR_OOM, T0B_ERR_DEVICE = range(7)
 F32, F16, Q4_0, Q8_0 = 0, 1, 2, 8
+BF16 = 30
+FP4_MX, FP4_NV = 1, 2
 
 # every symbol include/t0b.h declares
 EXPORTED = [
@@ -24,6 +26,8 @@ EXPORTED = [
     "t0b_gguf_validate",
     "t0b_quantize", "t0b_dequantize", "t0b_row_bytes", "t0b_export_gguf", "t0b_model_profile_enable",
     "t0b_model_profile_read", "t0b_model_launch_count", "t0b_selftest_bounded_wait",
+    "t0b_fp4_code_bytes", "t0b_fp4_scale_bytes", "t0b_fp4_quantize", "t0b_fp4_dequantize", "t0b_fp4_gemm",
+    "t0b_fp4_glu", "t0b_fp4_linear", "t0b_fp4_mlp", "t0b_fp4_sync",
 ]
 
 
@@ -40,6 +44,12 @@ class ModelInfo(C.Structure):
         ("scaler_use_arcsinh", C.c_int32), ("scaler_eps", C.c_float), ("variance_offset", C.c_int32),
         ("weight_type", C.c_int32), ("quantizable_gpu_bytes", C.c_uint64), ("total_weight_bytes", C.c_uint64),
     ]
+
+
+class Fp4(C.Structure):
+    """A matrix of 4-bit microscaled values (t0b_fp4)."""
+    _fields_ = [("format", C.c_int32), ("rows", C.c_int32), ("k", C.c_int32), ("tensor_scale", C.c_float),
+                ("codes", C.c_void_p), ("scales", C.c_void_p)]
 
 
 class T0bError(RuntimeError):
@@ -99,6 +109,18 @@ def lib() -> C.CDLL:
     L.t0b_model_launch_count.argtypes = [vp]
     L.t0b_model_launch_count.restype = C.c_uint64
     L.t0b_selftest_bounded_wait.argtypes = [vp, C.POINTER(C.c_int), C.POINTER(C.c_int)]
+    i64, f4 = C.c_int64, C.POINTER(Fp4)
+    L.t0b_fp4_code_bytes.argtypes = [st, st]
+    L.t0b_fp4_code_bytes.restype = sz
+    L.t0b_fp4_scale_bytes.argtypes = [st, st, st]
+    L.t0b_fp4_scale_bytes.restype = sz
+    L.t0b_fp4_quantize.argtypes = [vp, st, vp, i64, f4, vp]
+    L.t0b_fp4_dequantize.argtypes = [vp, f4, st, vp, i64, vp]
+    L.t0b_fp4_gemm.argtypes = [vp, f4, f4, vp, st, vp, i64, vp]
+    L.t0b_fp4_glu.argtypes = [vp, f4, f4, vp, st, vp, i64, f4, vp]
+    L.t0b_fp4_linear.argtypes = [vp, f4, st, vp, i64, f4, vp, st, vp, i64, vp]
+    L.t0b_fp4_mlp.argtypes = [vp, f4, f4, st, vp, i64, f4, f4, vp, vp, st, vp, i64, vp]
+    L.t0b_fp4_sync.argtypes = [vp, vp]
     _lib = L
     return L
 

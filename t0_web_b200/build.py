@@ -19,7 +19,7 @@ OBJ = os.path.join(HERE, "_build")
 LIB_CHECKED = os.path.join(HERE, "libt0b_checked.so")
 OBJ_CHECKED = os.path.join(HERE, "_build_checked")
 
-CU_SOURCES = ["t0b_model.cu", "k_gemm_small.cu", "k_gemm_tc.cu", "k_misc.cu"]
+CU_SOURCES = ["t0b_model.cu", "k_gemm_small.cu", "k_gemm_tc.cu", "k_misc.cu", "k_fp4.cu", "t0b_fp4.cu"]
 CPP_SOURCES = ["gguf_host.cpp"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 

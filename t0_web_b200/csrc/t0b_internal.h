@@ -116,3 +116,31 @@ cudaError_t t0b_launch_split_f32(const float *x, __half *xh, __half *xl, size_t 
 // Self-test of the bounded mbarrier wait (k_misc.cu): one warp waits on a
 // barrier nobody arrives on; *outcome = 2 once the wait ran out and returned.
 cudaError_t t0b_launch_bounded_wait_selftest(int *err, int *outcome, cudaStream_t st);
+
+// ---- 4-bit microscaled operators (k_fp4.cu; entry points in t0b_fp4.cu)
+struct t0b_engine;
+// Records `msg` as the calling thread's last error and returns `status`.
+int t0b_set_error(int status, const char *msg);
+int t0b_engine_device(const t0b_engine *e);
+int *t0b_engine_fp4_err(const t0b_engine *e);  // device error word of the 4-bit operators
+
+// A matrix of 4-bit values on the device (t0b.h: t0b_fp4); blk is 32 (scales
+// are powers of two) or 16 (scales are 4-exponent, 3-mantissa bit floats).
+struct Fp4Mat {
+  uint8_t *codes, *scales;
+  int rows, k, blk;
+  float ts;
+};
+// Where a product's result goes: y (ggml type `type`, rows ld elements apart)
+// or, for a gated product, the 4-bit matrix q.
+struct Fp4Out {
+  int type;
+  void *y;
+  int64_t ld;
+  const float *bias;
+  bool glu, quant;
+  Fp4Mat q;
+};
+cudaError_t t0b_launch_fp4_quantize(int x_type, const void *x, int64_t ldx, const Fp4Mat &out, cudaStream_t st);
+cudaError_t t0b_launch_fp4_dequantize(const Fp4Mat &in, int y_type, void *y, int64_t ldy, cudaStream_t st);
+cudaError_t t0b_launch_fp4_gemm(const Fp4Mat &w, const Fp4Mat &x, const Fp4Out &out, int *err, cudaStream_t st);

@@ -101,7 +101,7 @@ struct LayerW {
 
 struct t0b_engine {
   int device = 0;
-  int *d_err = nullptr;
+  int *d_err = nullptr;      // [0] the standalone GEMMs' error word, [1] the 4-bit operators'
   DBuf scratch_xh, scratch_xl, scratch_zh, scratch_zl, scratch_red;
 };
 
@@ -196,7 +196,7 @@ extern "C" t0b_status t0b_engine_create(int device, t0b_engine **out) {
                                          std::to_string(prop.major) + std::to_string(prop.minor));
   auto *e = new t0b_engine();
   e->device = device;
-  if (cudaMalloc(&e->d_err, sizeof(int)) != cudaSuccess || cudaMemset(e->d_err, 0, sizeof(int)) != cudaSuccess) {
+  if (cudaMalloc(&e->d_err, 2 * sizeof(int)) != cudaSuccess || cudaMemset(e->d_err, 0, 2 * sizeof(int)) != cudaSuccess) {
     delete e;
     return fail(T0B_ERR_OOM, "t0b_engine_create: device allocation failed");
   }
@@ -210,6 +210,11 @@ extern "C" void t0b_engine_destroy(t0b_engine *e) {
   if (e->d_err) cudaFree(e->d_err);
   delete e;
 }
+
+// What t0b_fp4.cu needs of this file.
+int t0b_set_error(int status, const char *msg) { return fail(status, msg); }
+int t0b_engine_device(const t0b_engine *e) { return e->device; }
+int *t0b_engine_fp4_err(const t0b_engine *e) { return e->d_err + 1; }
 
 // ==================================================================== model
 namespace {
