@@ -2,6 +2,9 @@
 // matrices (layout: t0b.h, t0b_fp4).
 #include <cuda_bf16.h>
 
+#include <map>
+#include <mutex>
+
 #include "common.cuh"
 #include "t0b_internal.h"
 
@@ -68,47 +71,92 @@ T0B_DEV float code_value(uint32_t c) {
   return c & 8 ? -v : v;
 }
 
+// A block's scale byte and the factors that divide by its scale, from the bits
+// of its largest magnitude (infinities and NaNs compare above every finite
+// value).  The quotients are correctly rounded, so that every rounding to 4
+// bits is decided as if it were exact: with power-of-two scales the product
+// with 1 / d is exact; otherwise d has four significant bits, a quotient that
+// is not itself a border differs from it by more than half an ulp, and one
+// residual step (x - u d is exact in an FMA, 1 / d correctly rounded) gives
+// the correctly rounded quotient.
+template <bool NV>
+struct BlockScale {
+  uint32_t byte;
+  float d, rcp;
+  bool clamp;  // quotients that may overflow (only where the scale is at its largest)
+  T0B_DEV BlockScale(uint32_t amax, float ts) {
+    clamp = false;
+    if constexpr (!NV) {
+      byte = amax >= 0x7F800000u ? 255u : max(amax >> 23, 2u) - 2u;
+      rcp = __uint_as_float((254u - min(byte, 252u)) << 23);
+      d = 0.0f;
+    } else {
+      const float a = __uint_as_float(amax);
+      byte = amax >= 0x7F800000u ? 127u : e4m3_of(__fdiv_rn(a, 6.0f * ts));
+      d = e4m3_value(byte) * ts;
+      rcp = byte ? __frcp_rn(d) : 0.0f;  // a scale of zero: all values zero
+      clamp = a > 16.0f * d && byte;
+    }
+  }
+  T0B_DEV float quotient(float x) const {
+    if constexpr (!NV) return x * rcp;
+    const float u = x * rcp;
+    return fmaf(-fmaf(u, d, -x), rcp, u);  // this order keeps the sign of a zero
+  }
+};
+
+// A block's values to codes, eight to a word.
+template <bool NV>
+T0B_DEV void quantize_block(const BlockScale<NV> &s, float *v, uint32_t *w) {
+  constexpr int BLK = NV ? 16 : 32;
+  if (s.clamp) {
+#pragma unroll
+    for (int i = 0; i < BLK; ++i) v[i] = fminf(fmaxf(v[i], -8.0f * s.d), 8.0f * s.d);
+  }
+#pragma unroll
+  for (int i = 0; i < BLK / 8; ++i) {
+    float u[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) u[j] = s.quotient(v[8 * i + j]);
+    if constexpr (NV) {
+      if (s.byte == 0)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) u[j] = 0.0f;  // no signs either
+    }
+    w[i] = codes4(u[0], u[1], u[2], u[3]) | codes4(u[4], u[5], u[6], u[7]) << 16;
+  }
+}
+
 // ------------------------------------------------------------ quantisation
 // One thread per block of values.
-template <int TY>
+template <int TY, bool NV>
 __global__ void fp4_quantize_kernel(const typename Plain<TY>::T *x, int64_t ldx, Fp4Mat q) {
-  const int kt = (q.k + 4 * q.blk - 1) / (4 * q.blk), nb = kt * 4;
+  constexpr int BLK = NV ? 16 : 32;
+  const int kt = (q.k + 4 * BLK - 1) / (4 * BLK), nb = kt * 4;
   const size_t id = blockIdx.x * (size_t)blockDim.x + threadIdx.x;
   const int r = (int)(id / nb), b = (int)(id % nb);
   if (r >= (q.rows + 127) / 128 * 128) return;
   uint8_t *sc = q.scales + scale_at(r, b, kt);
-  const int k0 = b * q.blk;
+  const int k0 = b * BLK;
+  uint8_t *c = q.codes + r * code_pitch(q.k) + k0 / 2;
   if (r >= q.rows || k0 >= q.k) {
     *sc = 0;
     // the second half of a 32-value group whose last block is missing
     if (r < q.rows && (size_t)k0 / 2 < code_pitch(q.k))
-      for (int i = 0; i < q.blk / 2; ++i) q.codes[r * code_pitch(q.k) + k0 / 2 + i] = 0;
+      for (int i = 0; i < BLK / 2; ++i) c[i] = 0;
     return;
   }
-  float v[32];
+  float v[BLK];
   uint32_t amax = 0;
-  for (int i = 0; i < q.blk; ++i) {
+  for (int i = 0; i < BLK; ++i) {
     v[i] = k0 + i < q.k ? Plain<TY>::get(x[r * ldx + k0 + i]) : 0.0f;
     amax = max(amax, __float_as_uint(v[i]) & 0x7FFFFFFFu);
   }
-  uint32_t byte;
-  float d;  // the block's scale
-  if (q.blk == 32) {
-    byte = amax >= 0x7F800000u ? 255u : max(amax >> 23, 2u) - 2u;
-    d = __uint_as_float(byte ? byte << 23 : 1u << 22);
-  } else {
-    byte = amax >= 0x7F800000u ? 127u : e4m3_of(__fdiv_rn(__uint_as_float(amax), 6.0f * q.ts));
-    d = e4m3_value(byte) * q.ts;
-  }
-  *sc = (uint8_t)byte;
-  uint8_t *c = q.codes + r * code_pitch(q.k) + k0 / 2;
-  for (int i = 0; i < q.blk; i += 4) {
-    float u[4];
-    for (int j = 0; j < 4; ++j) u[j] = byte == 0 && q.blk == 16 ? 0.0f : fminf(fmaxf(__fdiv_rn(v[i + j], d), -6.0f), 6.0f);
-    const uint32_t w = codes4(u[0], u[1], u[2], u[3]);
-    c[i / 2] = (uint8_t)w;
-    c[i / 2 + 1] = (uint8_t)(w >> 8);
-  }
+  const BlockScale<NV> s(amax, q.ts);
+  *sc = (uint8_t)s.byte;
+  uint32_t w[BLK / 8];
+  quantize_block<NV>(s, v, w);
+  for (int i = 0; i < BLK / 2; ++i) c[i] = (uint8_t)(w[i / 4] >> (i % 4 * 8));
 }
 
 template <int TY>
@@ -123,73 +171,394 @@ __global__ void fp4_dequantize_kernel(Fp4Mat q, typename Plain<TY>::T *y, int64_
   y[r * ldy + k] = Plain<TY>::put(code_value(c) * s * q.ts);
 }
 
-// One value per lane, 32 consecutive columns c0 .. c0 + 31 of row r (zeros
-// behind the matrix) to 4 bits: the block's largest magnitude by shuffles.
-// Every lane of the warp calls it; c0 is a multiple of 32.
-T0B_DEV void quantize_lanes(const Fp4Mat &q, int r, int c0, float v) {
-  const int lane = threadIdx.x & 31;
-  const int kt = (q.k + 4 * q.blk - 1) / (4 * q.blk);
-  uint32_t amax = r < q.rows ? __float_as_uint(v) & 0x7FFFFFFFu : 0;
-  for (int o = q.blk / 2; o; o >>= 1) amax = max(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, o));
-  uint32_t byte;
-  float d;
-  if (q.blk == 32) {
-    byte = amax >= 0x7F800000u ? 255u : max(amax >> 23, 2u) - 2u;
-    d = __uint_as_float(byte ? byte << 23 : 1u << 22);
-  } else {
-    byte = amax >= 0x7F800000u ? 127u : e4m3_of(__fdiv_rn(__uint_as_float(amax), 6.0f * q.ts));
-    d = e4m3_value(byte) * q.ts;
-  }
-  const int b = (c0 + lane) / q.blk;
-  if (b < 4 * kt && lane % q.blk == 0) q.scales[scale_at(r, b, kt)] = r < q.rows && b * q.blk < q.k ? (uint8_t)byte : 0;
-  float u = byte == 0 && q.blk == 16 ? 0.0f : fminf(fmaxf(__fdiv_rn(v, d), -6.0f), 6.0f);
-  const float u1 = __shfl_down_sync(0xFFFFFFFFu, u, 1);
-  if (r < q.rows && lane % 2 == 0 && (size_t)c0 / 2 < code_pitch(q.k))
-    q.codes[r * code_pitch(q.k) + (c0 + lane) / 2] = (uint8_t)codes4(u, u1, 0.0f, 0.0f);
-}
-
 // ----------------------------------------------------------------- product
-T0B_DEV float mat_at(const Fp4Mat &q, int r, int k, int kt) {
-  const uint32_t c = q.codes[r * code_pitch(q.k) + k / 2] >> (k % 2 * 4) & 15;
-  return code_value(c) * scale_value(q.blk, q.scales[scale_at(r, k / q.blk, kt)]);
+// silu(g) * u.  1 / (1 + exp(-g)) with exp as 2^t, t = -g log2(e) carried to
+// twice the precision (the rounding error of t would otherwise grow with g);
+// g is clamped where the sigmoid is 0 or 1 to the last bit.
+T0B_DEV float silu_mul(float g, float u) {
+  constexpr float L = 1.44269504f, L2 = 1.92596299e-8f, LN2 = 0.693147181f;
+  const float c = fminf(fmaxf(g, -126.0f), 126.0f);
+  const float t = -c * L;
+  const float e = fmaf(-c, L2, fmaf(-c, L, -t));  // the part of -c log2(e) that t lost
+  float p;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p) : "f"(t));
+  p *= fmaf(e, LN2, 1.0f);
+  float s;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(1.0f + p));
+  return g * s * u;
 }
 
-// One 32 x 32 tile of the result per CTA, one thread per value; with GLU two
-// sums per thread.
-template <int TY, bool GLU>
-__global__ void fp4_gemm_kernel(Fp4Mat w, Fp4Mat x, Fp4Out out, int n) {
-  __shared__ float xs[32][33], ws[32][33], us[32][33];
-  const int tx = threadIdx.x, ty = threadIdx.y;
-  const int r = blockIdx.y * 32 + ty, c = blockIdx.x * 32 + tx;
-  const int kt = (w.k + 4 * w.blk - 1) / (4 * w.blk);
-  float acc = 0.0f, acu = 0.0f;
-  for (int k0 = 0; k0 < w.k; k0 += 32) {
-    const bool kin = k0 + tx < w.k;
-    const int wr = blockIdx.x * 32 + ty;
-    xs[ty][tx] = kin && r < x.rows ? mat_at(x, r, k0 + tx, kt) : 0.0f;
-    ws[ty][tx] = kin && wr < n ? mat_at(w, wr, k0 + tx, kt) : 0.0f;
-    if (GLU) us[ty][tx] = kin && wr < n ? mat_at(w, wr + n, k0 + tx, kt) : 0.0f;
-    __syncthreads();
-    for (int k = 0; k < 32; ++k) {
-      acc = fmaf(xs[ty][k], ws[tx][k], acc);
-      if (GLU) acu = fmaf(xs[ty][k], us[tx][k], acu);
+// 32 accumulator columns of this thread's lane; the values may be used after
+// tmem_ld_wait on them.
+T0B_DEV void tmem_ld32(uint32_t addr, uint32_t *r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,"
+      "%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(addr));
+}
+T0B_DEV void tmem_ld_wait(uint32_t *r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                 "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]),
+                 "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
+                 "+r"(r[30]), "+r"(r[31])::"memory");
+}
+T0B_DEV void tma_load_3d_pair(void *dst, const void *tmap, uint32_t bar_cl, int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, "
+      "%5}], [%2];" ::"r"(smem_u32(dst)),
+      "l"((uint64_t)tmap), "r"(bar_cl), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+// Shared-memory descriptor of a K-major tile of 128-byte rows (256 4-bit
+// values) with the 128-byte swizzle: 8-row atoms of 1024 bytes.
+T0B_DEV uint64_t sw128_desc(uint32_t saddr) {
+  return (uint64_t)((saddr & 0x3FFFFu) >> 4) | (uint64_t)1 << 16 | (uint64_t)(1024u >> 4) << 32 | (uint64_t)1 << 46 |
+         (uint64_t)2 << 61;
+}
+// A 512-byte scale tile (32 rows of 16 bytes, no swizzle), for tcgen05.cp.
+T0B_DEV uint64_t scale_desc(uint32_t saddr) {
+  return (uint64_t)((saddr & 0x3FFFFu) >> 4) | (uint64_t)1 << 16 | (uint64_t)(128u >> 4) << 32 | (uint64_t)1 << 46;
+}
+// Copies a scale tile into four TMEM columns, the 32 rows repeated in the four
+// lane quarters, in both CTAs of a pair (each from its own shared memory).
+T0B_DEV void scale_cp_pair(uint32_t taddr, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+// Instruction descriptor of the block-scaled 4-bit product: e2m1 A and B
+// (format 1), scales as unsigned e4m3 (NV) or powers of two, M x N, K-major.
+template <bool NV>
+__host__ __device__ constexpr uint32_t idesc_fp4(int M, int N) {
+  return 1u << 7 | 1u << 10 | (uint32_t)(N >> 3) << 17 | (NV ? 0u : 1u) << 23 | (uint32_t)(M >> 4) << 24;
+}
+// Which bytes of the scale words a K = 64 step uses (blocks of 32: two of the
+// four, so steps alternate; blocks of 16: all four).
+T0B_DEV uint32_t idesc_scale_id(uint32_t id) { return id << 4 | id << 29; }
+template <bool NV>
+T0B_DEV void umma_fp4_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t acc) {
+  if constexpr (NV)
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %6, 0;\n"
+        " tcgen05.mma.cta_group::2.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(acc)
+        : "memory");
+  else
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %6, 0;\n"
+        " tcgen05.mma.cta_group::2.kind::mxf4nvf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(acc)
+        : "memory");
+}
+
+// Arguments of the product kernels beside the tensor maps.
+struct Fp4Args {
+  int M, n, K;     // tokens, result columns (a gated product's F), values
+  int kt;          // scale tiles along K
+  float alpha;     // product of the tensor scales
+  const float *bias;
+  void *y;
+  int64_t ld;
+  Fp4Mat q;        // the 4-bit result, where the kernel quantises it
+  int up_row;      // gated: first up row (F)
+  int n_tiles_n, n_tiles;
+  bool vec;        // rows of y can be written in 16-byte pieces
+  int *err;
+};
+
+// The product on CTA pairs (cta_group::2): 256 tokens x 256 weight rows a
+// tile, one M = 256, N = 256, K = 64 block-scaled MMA over both CTAs'
+// tiles of codes per step; CTA r holds tokens 128 r .. of the tile and weight
+// rows 128 r .. (gated: CTA 0 gate rows, CTA 1 the matching up rows), and the
+// scales of its tokens and of all 256 weight rows.
+constexpr int PAIR_EPI_WARPS = 8;
+constexpr int PAIR_THREADS = 128 + 32 * PAIR_EPI_WARPS;
+
+template <bool NV, bool ROT>
+struct PairCfg {
+  static constexpr int AT = NV ? 4 : 2;                    // scale tiles of a 256-value stage
+  static constexpr uint32_t CODES = 128 * 128;             // one operand's codes of a stage
+  static constexpr uint32_t SC = AT * 512;                 // 128 rows' scales of a stage
+  static constexpr uint32_t STAGE = 2 * CODES + (ROT ? 5 : 3) * SC;
+  static constexpr int NS = 5;                             // stages
+  static constexpr uint32_t OFF_A = 0, OFF_B = CODES, OFF_SA = 2 * CODES, OFF_SB = OFF_SA + SC, OFF_RAW = OFF_SB + 2 * SC;
+  static constexpr uint32_t OFF_BIAS = NS * STAGE, OFF_BAR = OFF_BIAS + 256 * 4, SMEM = OFF_BAR + 256 + 1024;
+  static constexpr uint32_t SFC = AT * 12;                 // TMEM columns of a stage's scales
+  static_assert(256 + NS * SFC <= 512, "accumulator and scales in TMEM");
+  static_assert(STAGE % 1024 == 0 && SMEM <= 232448, "shared memory");
+};
+
+// 32 consecutive values of row r, columns c0 .. (a multiple of 32), to 4 bits;
+// values behind the matrix are taken as zero and its padding is written.
+template <bool NV>
+T0B_DEV void store_quant32(const Fp4Mat &q, int r, int c0, float *v) {
+  constexpr int BLK = NV ? 16 : 32, NB = 32 / BLK;
+  const int kt = (q.k + 4 * BLK - 1) / (4 * BLK);
+  if (r >= (q.rows + 127) / 128 * 128 || c0 >= kt * 4 * BLK) return;
+#pragma unroll
+  for (int j = 0; j < 32; ++j)
+    if (r >= q.rows || c0 + j >= q.k) v[j] = 0.0f;
+  uint32_t w[4], sc = 0;
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    uint32_t amax = 0;
+#pragma unroll
+    for (int j = 0; j < BLK; ++j) amax = max(amax, __float_as_uint(v[b * BLK + j]) & 0x7FFFFFFFu);
+    const BlockScale<NV> s(amax, q.ts);
+    sc |= s.byte << (8 * b);
+    quantize_block<NV>(s, v + b * BLK, w + b * BLK / 8);
+  }
+  uint8_t *ps = q.scales + scale_at(r, c0 / BLK, kt);
+  if (NV)
+    *reinterpret_cast<uint16_t *>(ps) = (uint16_t)sc;
+  else
+    *ps = (uint8_t)sc;
+  if (r < q.rows && c0 < q.k) *reinterpret_cast<uint4 *>(q.codes + r * code_pitch(q.k) + c0 / 2) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Writes 32 consecutive values of one row, columns c0 .. of n.
+template <int TY>
+T0B_DEV void store_row32(const Fp4Args &p, int m, int c0, const float *v) {
+  using T = typename Plain<TY>::T;
+  T *dst = reinterpret_cast<T *>(p.y) + m * p.ld + c0;
+  if (p.vec && c0 + 32 <= p.n) {
+    constexpr int PER = 16 / sizeof(T);
+#pragma unroll
+    for (int i = 0; i < 32 / PER; ++i) {
+      alignas(16) T t[PER];
+#pragma unroll
+      for (int j = 0; j < PER; ++j) t[j] = Plain<TY>::put(v[i * PER + j]);
+      reinterpret_cast<uint4 *>(dst)[i] = *reinterpret_cast<const uint4 *>(t);
     }
-    __syncthreads();
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (c0 + j < p.n) dst[j] = Plain<TY>::put(v[j]);
   }
-  const bool live = r < x.rows && c < n;
-  if (!live && !out.quant) return;
-  acc = acc * (w.ts * x.ts) + (live && out.bias ? out.bias[c] : 0.0f);
-  if (GLU) {
-    acu = acu * (w.ts * x.ts) + (live && out.bias ? out.bias[c + n] : 0.0f);
-    acc = acc / (1.0f + expf(-acc)) * acu;
-  }
-  if (out.quant) {
-    quantize_lanes(out.q, r, blockIdx.x * 32, live ? acc : 0.0f);
+}
+
+// TY: result type, or -1 for the 4-bit result of a gated product.
+template <bool NV, bool GLU, bool ROT, int TY>
+__global__ void __launch_bounds__(PAIR_THREADS, 1)
+    fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
+                         const __grid_constant__ CUtensorMap tm_xs, const __grid_constant__ CUtensorMap tm_ws, Fp4Args p) {
+  using C = PairCfg<NV, ROT>;
+  constexpr int AT = C::AT, NS = C::NS;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t *smem = smem_raw + (base - smem_u32(smem_raw));
+  if (cluster_size() != 2) {
+    if (threadIdx.x == 0) record_error(p.err, T0B_DEVERR_SHAPE);
     return;
   }
-  reinterpret_cast<typename Plain<TY>::T *>(out.y)[r * out.ld + c] = Plain<TY>::put(acc);
+  const uint32_t rank = cluster_rank();
+  uint64_t *full = reinterpret_cast<uint64_t *>(smem + C::OFF_BAR);  // [NS] bytes of both CTAs (CTA 0's)
+  uint64_t *empty = full + NS;       // [NS] the stage's MMAs are done (each CTA's)
+  uint64_t *raw_full = empty + NS;   // [NS] up rows' scales as they are held (each CTA's; ROT)
+  uint64_t *rot_full = raw_full + NS;  // [NS] and moved to the tile's rows, both CTAs (CTA 0's; ROT)
+  uint64_t *acc_full = rot_full + NS;  // each CTA's
+  uint64_t *acc_empty = acc_full + 1;  // epilogue warps of both CTAs (CTA 0's)
+  uint64_t *mma_done = acc_empty + 1;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(mma_done + 1);
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(mma_done + 2);
+  float *sbias = reinterpret_cast<float *>(smem + C::OFF_BIAS);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int S = (p.K + 255) / 256;
+  const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < NS; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+      mbar_init(&raw_full[i], 1);
+      mbar_init(&rot_full[i], 2);
+    }
+    mbar_init(acc_full, 1);
+    mbar_init(acc_empty, 2 * PAIR_EPI_WARPS);
+    mbar_init(mma_done, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+    fence_proxy_async_smem();
+    prefetch_tmap(&tm_x);
+    prefetch_tmap(&tm_w);
+    prefetch_tmap(&tm_xs);
+    prefetch_tmap(&tm_ws);
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(tmem_slot, 512);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  auto lead = [](const uint64_t *b) { return mapa_shared(smem_u32(b), 0); };
+  // first weight row of this CTA's half, and of each half's scales
+  auto w_row = [&](int nt, uint32_t half) { return GLU ? nt * 128 + (half ? p.up_row : 0) : nt * 256 + 128 * (int)half; };
+
+  if (warp == 0 && lane == 0) {
+    // ------------------------------------------------------------ loads (both CTAs)
+    uint32_t g = 0;
+    pdl_wait();
+    for (int tile = pair; tile < p.n_tiles && !*abort_flag; tile += npairs) {
+      const int nt = tile % p.n_tiles_n, m0 = tile / p.n_tiles_n * 256 + 128 * (int)rank;
+      for (int s = 0; s < S && !*abort_flag; ++s, ++g) {
+        const uint32_t sl = g % NS;
+        if (g >= NS && !mbar_wait(&empty[sl], (g / NS - 1) & 1, p.err, T0B_DEVERR_WAIT_EMPTY, abort_flag)) break;
+        uint8_t *st = smem + sl * C::STAGE;
+        if (rank == 0) mbar_arrive_expect_tx(&full[sl], 4 * C::CODES + (ROT ? 4 : 6) * C::SC);
+        const uint32_t fb = lead(&full[sl]);
+        // (byte, row) of the codes, (tile, row group) of the scales; what lies
+        // behind the matrix arrives as zeros
+        tma_load_2d_pair(st + C::OFF_A, &tm_x, fb, s * 128, m0);
+        tma_load_2d_pair(st + C::OFF_B, &tm_w, fb, s * 128, w_row(nt, rank));
+        tma_load_3d_pair(st + C::OFF_SA, &tm_xs, fb, 0, s * AT, m0 >> 7);
+        tma_load_3d_pair(st + C::OFF_SB, &tm_ws, fb, 0, s * AT, w_row(nt, 0) >> 7);
+        if constexpr (!ROT) {
+          tma_load_3d_pair(st + C::OFF_SB + C::SC, &tm_ws, fb, 0, s * AT, w_row(nt, 1) >> 7);
+        } else {
+          mbar_arrive_expect_tx(&raw_full[sl], 2 * C::SC);
+          tma_load_3d(st + C::OFF_RAW, &tm_ws, &raw_full[sl], 0, s * AT, w_row(nt, 1) >> 7);
+          tma_load_3d(st + C::OFF_RAW + C::SC, &tm_ws, &raw_full[sl], 0, s * AT, (w_row(nt, 1) >> 7) + 1);
+        }
+      }
+    }
+  } else if (warp == 1 && lane == 0 && rank == 0) {
+    // ------------------------------------------------------------ MMA (CTA 0)
+    constexpr uint32_t idesc = idesc_fp4<NV>(256, 256);
+    uint32_t g = 0, it = 0;
+    const int steps = (p.K + 63) / 64;
+    for (int tile = pair; tile < p.n_tiles && !*abort_flag; tile += npairs, ++it) {
+      if (it >= 1 && !mbar_wait(acc_empty, (it - 1) & 1, p.err, T0B_DEVERR_WAIT_ACC, abort_flag)) break;
+      tc_fence_after();
+      for (int s = 0; s < S; ++s, ++g) {
+        const uint32_t sl = g % NS;
+        if (!mbar_wait(&full[sl], (g / NS) & 1, p.err, T0B_DEVERR_WAIT_X, abort_flag)) break;
+        if (ROT && !mbar_wait(&rot_full[sl], (g / NS) & 1, p.err, T0B_DEVERR_WAIT_DEQ, abort_flag)) break;
+        tc_fence_after();
+        const uint32_t st = base + sl * C::STAGE, sf = tmem + 256 + sl * C::SFC;
+#pragma unroll
+        for (int a = 0; a < AT; ++a) {
+          scale_cp_pair(sf + 4 * a, scale_desc(st + C::OFF_SA + 512 * a));
+          scale_cp_pair(sf + 4 * AT + 8 * a, scale_desc(st + C::OFF_SB + 512 * a));
+          scale_cp_pair(sf + 4 * AT + 8 * a + 4, scale_desc(st + C::OFF_SB + C::SC + 512 * a));
+        }
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+          if (4 * s + kk >= steps) break;
+          const int a = NV ? kk : kk / 2;
+          umma_fp4_pair<NV>(tmem, sw128_desc(st + C::OFF_A + 32 * kk), sw128_desc(st + C::OFF_B + 32 * kk),
+                            idesc | (NV ? 0u : idesc_scale_id(kk % 2 * 2)), sf + 4 * a, sf + 4 * AT + 8 * a,
+                            s > 0 || kk > 0);
+        }
+        umma_commit_pair_both(&empty[sl]);
+      }
+      if (*abort_flag) break;
+      umma_commit_pair_both(acc_full);
+    }
+    umma_commit_pair(smem_u32(mma_done));
+    mbar_wait(mma_done, 0, p.err, T0B_DEVERR_WAIT_ACC, nullptr);
+  } else if (ROT && warp == 2) {
+    // ------------------------------------------------------------ up rows' scales (both CTAs)
+    // The scale tiles hold 128 rows from a multiple of 128 on; the up rows of
+    // a tile start at F + f0.  Moves them to their place in the tile.
+    uint32_t g = 0;
+    const int off = p.up_row & 127;
+    bool ok = true;
+    for (int tile = pair; tile < p.n_tiles && ok && !*abort_flag; tile += npairs) {
+      for (int s = 0; s < S; ++s, ++g) {
+        const uint32_t sl = g % NS;
+        bool got = true;
+        if (lane == 0) got = mbar_wait(&raw_full[sl], (g / NS) & 1, p.err, T0B_DEVERR_WAIT_W, abort_flag);
+        if (!__shfl_sync(0xFFFFFFFFu, got ? 1 : 0, 0)) {
+          ok = false;
+          break;
+        }
+        const uint32_t *raw = reinterpret_cast<const uint32_t *>(smem + sl * C::STAGE + C::OFF_RAW);
+        uint32_t *dst = reinterpret_cast<uint32_t *>(smem + sl * C::STAGE + C::OFF_SB + C::SC);
+#pragma unroll
+        for (int a = 0; a < AT; ++a)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int r = off + 32 * j + lane;
+            dst[a * 128 + lane * 4 + j] = raw[(r >> 7) * (AT * 128) + a * 128 + (r & 31) * 4 + ((r >> 5) & 3)];
+          }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(lead(&rot_full[sl]));
+      }
+    }
+  } else if (warp >= 4) {
+    // ------------------------------------------------------------ epilogue (both CTAs)
+    const int q = warp & 3, h = (warp - 4) >> 2;  // lane quarter, column half
+    const int et = threadIdx.x - 128;
+    uint32_t it = 0;
+    for (int tile = pair; tile < p.n_tiles; tile += npairs, ++it) {
+      const int nt = tile % p.n_tiles_n, m0 = tile / p.n_tiles_n * 256 + 128 * (int)rank;
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      {
+        const int col = GLU ? nt * 128 + (et & 127) : nt * 256 + et;
+        sbias[et] = p.bias && col < p.n ? p.bias[GLU && et >= 128 ? p.n + col : col] : 0.0f;
+      }
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      const int m = m0 + 32 * q + lane;
+      const uint32_t trow = tmem + ((uint32_t)(32 * q) << 16);
+      bool have = mbar_wait(acc_full, it & 1, p.err, T0B_DEVERR_WAIT_ACC, abort_flag) && !*abort_flag;
+      have = __all_sync(0xFFFFFFFFu, have);
+      tc_fence_after();
+      uint32_t r[4][32];  // 128 columns (gated: 64 gate, 64 up)
+      if (have) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) tmem_ld32(trow + (GLU ? 64 * h + 128 * (i >> 1) + 32 * (i & 1) : 128 * h + 32 * i), r[i]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) tmem_ld_wait(r[i]);
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(lead(acc_empty));
+      if (!have) continue;
+      if constexpr (!GLU) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int c0 = 128 * h + 32 * i;
+          float *v = reinterpret_cast<float *>(r[i]);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = fmaf(__uint_as_float(r[i][j]), p.alpha, sbias[c0 + j]);
+          if (m < p.M && nt * 256 + c0 < p.n) store_row32<TY < 0 ? TY_F32 : TY>(p, m, nt * 256 + c0, v);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int c0 = 64 * h + 32 * i, f0 = nt * 128 + c0;
+          float v[32];
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            v[j] = silu_mul(fmaf(__uint_as_float(r[i][j]), p.alpha, sbias[c0 + j]),
+                            fmaf(__uint_as_float(r[2 + i][j]), p.alpha, sbias[128 + c0 + j]));
+          if constexpr (TY >= 0) {
+            if (m < p.M && f0 < p.n) store_row32<TY < 0 ? TY_F32 : TY>(p, m, f0, v);
+          } else {
+            store_quant32<NV>(p.q, m, f0, v);
+          }
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem, 512);
+  }
 }
 
+// ------------------------------------------------------------- host side
 template <typename... P, typename... A>
 cudaError_t launch(void (*k)(P...), dim3 grid, dim3 block, cudaStream_t st, A... args) {
   cudaLaunchConfig_t cfg{};
@@ -199,14 +568,98 @@ cudaError_t launch(void (*k)(P...), dim3 grid, dim3 block, cudaStream_t st, A...
   return cudaLaunchKernelEx(&cfg, k, args...);
 }
 
+// Tensor maps of a matrix: codes in boxes of 128 rows x 128 bytes, scales in
+// boxes of one row group's `at` tiles.
+bool code_map(CUtensorMap *tm, const Fp4Mat &q) {
+  const uint64_t pitch = (uint64_t)((q.k + 31) / 32) * 16;
+  return t0b_make_tmap_u8_2d(tm, q.codes, pitch, (uint64_t)q.rows, pitch, 128, 128);
+}
+bool scale_map(CUtensorMap *tm, const Fp4Mat &q, int kt, int at) {
+  return t0b_make_tmap_f16_3d(tm, q.scales, 256, (uint64_t)kt, (uint64_t)((q.rows + 127) / 128), 512, (uint64_t)kt * 512, 256,
+                              (uint32_t)at, 1, false);
+}
+
+// Pairs of the kernel that fit on the current device at once, asked once per
+// kernel and device.
+int max_pairs(const void *kfn, const cudaLaunchConfig_t &cfg) {
+  static std::mutex mu;
+  static std::map<std::pair<const void *, int>, int> cache;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  std::lock_guard<std::mutex> lk(mu);
+  int &n = cache[{kfn, dev}];
+  if (n) return n;
+  int sms = 0;
+  if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+  cudaLaunchConfig_t c = cfg;
+  c.gridDim = dim3(sms / 2 * 2);
+  if (cudaOccupancyMaxActiveClusters(&n, kfn, &c) != cudaSuccess) {
+    cudaGetLastError();
+    n = 0;
+  }
+  return n;
+}
+
+template <bool NV, bool GLU, bool ROT, int TY>
+cudaError_t launch_pair(const Fp4Mat &w, const Fp4Mat &x, Fp4Args p, cudaStream_t st) {
+  using C = PairCfg<NV, ROT>;
+  auto kfn = fp4_gemm_pair_kernel<NV, GLU, ROT, TY>;
+  cudaError_t e = t0b_smem_limit((const void *)kfn, C::SMEM);
+  if (e != cudaSuccess) return e;
+  CUtensorMap tx, tw, txs, tws;
+  if (!code_map(&tx, x) || !code_map(&tw, w) || !scale_map(&txs, x, p.kt, C::AT) || !scale_map(&tws, w, p.kt, C::AT))
+    return cudaErrorInvalidValue;
+  p.n_tiles_n = GLU ? (p.n + 127) / 128 : (p.n + 255) / 256;
+  const int64_t tiles = (int64_t)p.n_tiles_n * ((p.M + 255) / 256);
+  if (tiles > INT32_MAX / 2) return cudaErrorInvalidValue;
+  p.n_tiles = (int)tiles;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = 2;
+  at[0].val.clusterDim.y = 1;
+  at[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.blockDim = dim3(PAIR_THREADS);
+  cfg.dynamicSmemBytes = C::SMEM;
+  cfg.stream = st;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  const int pairs = max_pairs((const void *)kfn, cfg);
+  if (pairs < 1) return cudaErrorInvalidConfiguration;
+  cfg.gridDim = dim3(2 * (p.n_tiles < pairs ? p.n_tiles : pairs));
+  return cudaLaunchKernelEx(&cfg, kfn, tx, tw, txs, tws, p);
+}
+
+template <bool NV, int TY>
+cudaError_t gemm_ty(const Fp4Mat &w, const Fp4Mat &x, const Fp4Out &out, const Fp4Args &p, cudaStream_t st) {
+  if (!out.glu) return launch_pair<NV, false, false, TY < 0 ? TY_F32 : TY>(w, x, p, st);
+  // gate and up rows meet in one tile; up rows that do not start at a row group's first row need their scales moved
+  return p.up_row % 128 ? launch_pair<NV, true, true, TY>(w, x, p, st) : launch_pair<NV, true, false, TY>(w, x, p, st);
+}
+
+template <bool NV>
+cudaError_t gemm_fmt(const Fp4Mat &w, const Fp4Mat &x, const Fp4Out &out, const Fp4Args &p, cudaStream_t st) {
+  if (out.quant) return gemm_ty<NV, -1>(w, x, out, p, st);
+  if (out.type == TY_F32) return gemm_ty<NV, TY_F32>(w, x, out, p, st);
+  if (out.type == TY_F16) return gemm_ty<NV, TY_F16>(w, x, out, p, st);
+  return gemm_ty<NV, TY_BF16>(w, x, out, p, st);
+}
+
+template <int TY>
+cudaError_t quantize_ty(const void *x, int64_t ldx, const Fp4Mat &q, cudaStream_t st) {
+  using T = typename Plain<TY>::T;
+  const size_t n = (size_t)((q.rows + 127) / 128 * 128) * ((q.k + 4 * q.blk - 1) / (4 * q.blk) * 4);
+  const dim3 grid((unsigned)((n + 127) / 128));
+  return q.blk == 16 ? launch(fp4_quantize_kernel<TY, true>, grid, 128, st, (const T *)x, ldx, q)
+                     : launch(fp4_quantize_kernel<TY, false>, grid, 128, st, (const T *)x, ldx, q);
+}
+
 }  // namespace
 
 cudaError_t t0b_launch_fp4_quantize(int x_type, const void *x, int64_t ldx, const Fp4Mat &q, cudaStream_t st) {
-  const size_t n = (size_t)((q.rows + 127) / 128 * 128) * ((q.k + 4 * q.blk - 1) / (4 * q.blk) * 4);
-  const dim3 grid((unsigned)((n + 127) / 128));
-  if (x_type == TY_F32) return launch(fp4_quantize_kernel<TY_F32>, grid, 128, st, (const float *)x, ldx, q);
-  if (x_type == TY_F16) return launch(fp4_quantize_kernel<TY_F16>, grid, 128, st, (const __half *)x, ldx, q);
-  return launch(fp4_quantize_kernel<TY_BF16>, grid, 128, st, (const __nv_bfloat16 *)x, ldx, q);
+  if (x_type == TY_F32) return quantize_ty<TY_F32>(x, ldx, q, st);
+  if (x_type == TY_F16) return quantize_ty<TY_F16>(x, ldx, q, st);
+  return quantize_ty<TY_BF16>(x, ldx, q, st);
 }
 
 cudaError_t t0b_launch_fp4_dequantize(const Fp4Mat &q, int y_type, void *y, int64_t ldy, cudaStream_t st) {
@@ -216,20 +669,20 @@ cudaError_t t0b_launch_fp4_dequantize(const Fp4Mat &q, int y_type, void *y, int6
   return launch(fp4_dequantize_kernel<TY_BF16>, grid, 128, st, q, (__nv_bfloat16 *)y, ldy);
 }
 
-template <int TY>
-static cudaError_t gemm_ty(const Fp4Mat &w, const Fp4Mat &x, const Fp4Out &out, cudaStream_t st) {
-  const int n = out.glu ? w.rows / 2 : w.rows;
-  // a 4-bit result: the scale tiles' rows and blocks behind the matrix too
-  const int cols = out.quant ? (n + 4 * w.blk - 1) / (4 * w.blk) * 4 * w.blk : n;
-  const int rows = out.quant ? (x.rows + 127) / 128 * 128 : x.rows;
-  const dim3 grid((cols + 31) / 32, (rows + 31) / 32), block(32, 32);
-  return out.glu ? launch(fp4_gemm_kernel<TY, true>, grid, block, st, w, x, out, n)
-                 : launch(fp4_gemm_kernel<TY, false>, grid, block, st, w, x, out, n);
-}
-
 cudaError_t t0b_launch_fp4_gemm(const Fp4Mat &w, const Fp4Mat &x, const Fp4Out &out, int *err, cudaStream_t st) {
-  (void)err;
-  if (out.type == TY_F32) return gemm_ty<TY_F32>(w, x, out, st);
-  if (out.type == TY_F16) return gemm_ty<TY_F16>(w, x, out, st);
-  return gemm_ty<TY_BF16>(w, x, out, st);
+  Fp4Args p{};
+  p.M = x.rows;
+  p.n = out.glu ? w.rows / 2 : w.rows;
+  p.K = w.k;
+  p.kt = (w.k + 4 * w.blk - 1) / (4 * w.blk);
+  p.alpha = w.ts * x.ts;
+  p.bias = out.bias;
+  p.y = out.y;
+  p.ld = out.ld;
+  p.q = out.q;
+  p.up_row = out.glu ? p.n : 0;
+  p.err = err;
+  const int es = out.type == TY_F32 ? 4 : 2;
+  p.vec = !out.quant && (uintptr_t)out.y % 16 == 0 && out.ld * es % 16 == 0;
+  return w.blk == 16 ? gemm_fmt<true>(w, x, out, p, st) : gemm_fmt<false>(w, x, out, p, st);
 }

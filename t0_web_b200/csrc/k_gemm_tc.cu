@@ -865,6 +865,14 @@ bool t0b_make_tmap_f32_2d(CUtensorMap *tm, const float *ptr, uint64_t inner, uin
                       swizzle128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
+// Byte tensor [outer][inner], box [box_outer][box_inner] with the 128-byte
+// swizzle: the 4-bit operators' code tiles.
+bool t0b_make_tmap_u8_2d(CUtensorMap *tm, const void *ptr, uint64_t inner, uint64_t outer, uint64_t row_bytes,
+                         uint32_t box_inner, uint32_t box_outer) {
+  return make_tmap_2d(tm, CU_TENSOR_MAP_DATA_TYPE_UINT8, ptr, inner, outer, row_bytes, box_inner, box_outer,
+                      CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
 // f16 tensor of dims {d0, d1, d2} (innermost first; d1 rows s1 bytes apart,
 // d2 slabs s2 bytes apart), box {b0, b1, b2}, optionally with the 128-byte
 // swizzle: for the attention kernels' TMA stores.
