@@ -39,14 +39,14 @@ T0B_DEV size_t code_pitch(int k) { return (size_t)((k + 31) / 32) * 16; }
 T0B_DEV size_t scale_at(int r, int b, int kt) {
   return ((size_t)(r >> 7) * kt + (b >> 2)) * 512 + (r & 31) * 16 + ((r >> 5) & 3) * 4 + (b & 3);
 }
-// Four values, already divided by their scale, to 4 bits each (first value
+// Eight values, already divided by their scale, to 4 bits each (first value
 // lowest): rounded to nearest, ties to the even index, at most 6.
-T0B_DEV uint32_t codes4(float a, float b, float c, float d) {
+T0B_DEV uint32_t codes8(const float *v) {
   uint32_t r;
-  asm("{\n .reg .b8 lo, hi;\n .reg .b16 w;\n cvt.rn.satfinite.e2m1x2.f32 lo, %2, %1;\n cvt.rn.satfinite.e2m1x2.f32 hi, %4, "
-      "%3;\n mov.b16 w, {lo, hi};\n cvt.u32.u16 %0, w;\n}"
+  asm("{\n .reg .b8 a, b, c, d;\n cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n"
+      " cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n mov.b32 %0, {a, b, c, d};\n}"
       : "=r"(r)
-      : "f"(a), "f"(b), "f"(c), "f"(d));
+      : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
   return r;
 }
 // f32 >= 0 to an unsigned 4-exponent, 3-mantissa bit float: nearest, ties to
@@ -61,14 +61,24 @@ T0B_DEV float e4m3_value(uint32_t b) {
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h2) : "h"((uint16_t)b));
   return __half2float(__ushort_as_half((uint16_t)h2));
 }
-T0B_DEV float scale_value(int blk, uint32_t byte) {
-  if (blk == 16) return e4m3_value(byte);
+template <bool NV>
+T0B_DEV float scale_value(uint32_t byte) {
+  if constexpr (NV) return e4m3_value(byte);
   return byte == 255 ? __uint_as_float(0x7FFFFFFFu) : __uint_as_float(byte ? byte << 23 : 1u << 22);
 }
-T0B_DEV float code_value(uint32_t c) {
-  const uint32_t m = c & 7;
-  const float v = m < 2 ? 0.5f * m : __uint_as_float(((126 + (m >> 1)) << 23) | ((m & 1) << 22));
-  return c & 8 ? -v : v;
+// Eight codes (first value lowest) to their values without scale.
+T0B_DEV void values8(uint32_t w, float *v) {
+  uint32_t h[4];
+  asm("{\n .reg .b8 a, b, c, d;\n mov.b32 {a, b, c, d}, %4;\n cvt.rn.f16x2.e2m1x2 %0, a;\n cvt.rn.f16x2.e2m1x2 %1, b;\n"
+      " cvt.rn.f16x2.e2m1x2 %2, c;\n cvt.rn.f16x2.e2m1x2 %3, d;\n}"
+      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+      : "r"(w));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h[i]));
+    v[2 * i] = f.x;
+    v[2 * i + 1] = f.y;
+  }
 }
 
 // A block's scale byte and the factors that divide by its scale, from the bits
@@ -105,70 +115,138 @@ struct BlockScale {
   }
 };
 
-// A block's values to codes, eight to a word.
+// Eight values of a block to a word of codes.
 template <bool NV>
-T0B_DEV void quantize_block(const BlockScale<NV> &s, float *v, uint32_t *w) {
-  constexpr int BLK = NV ? 16 : 32;
-  if (s.clamp) {
+T0B_DEV void quantize8(const BlockScale<NV> &s, const float *v, uint32_t *w) {
+  float u[8];
 #pragma unroll
-    for (int i = 0; i < BLK; ++i) v[i] = fminf(fmaxf(v[i], -8.0f * s.d), 8.0f * s.d);
+  for (int j = 0; j < 8; ++j) u[j] = s.quotient(v[j]);
+  if constexpr (NV) {
+    if (s.clamp)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) u[j] = s.quotient(fminf(fmaxf(v[j], -8.0f * s.d), 8.0f * s.d));
+    if (s.byte == 0)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) u[j] = 0.0f;  // no signs either
   }
-#pragma unroll
-  for (int i = 0; i < BLK / 8; ++i) {
-    float u[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) u[j] = s.quotient(v[8 * i + j]);
-    if constexpr (NV) {
-      if (s.byte == 0)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) u[j] = 0.0f;  // no signs either
-    }
-    w[i] = codes4(u[0], u[1], u[2], u[3]) | codes4(u[4], u[5], u[6], u[7]) << 16;
-  }
+  *w = codes8(u);
 }
 
 // ------------------------------------------------------------ quantisation
-// One thread per block of values.
-template <int TY, bool NV>
-__global__ void fp4_quantize_kernel(const typename Plain<TY>::T *x, int64_t ldx, Fp4Mat q) {
-  constexpr int BLK = NV ? 16 : 32;
-  const int kt = (q.k + 4 * BLK - 1) / (4 * BLK), nb = kt * 4;
-  const size_t id = blockIdx.x * (size_t)blockDim.x + threadIdx.x;
-  const int r = (int)(id / nb), b = (int)(id % nb);
-  if (r >= (q.rows + 127) / 128 * 128) return;
-  uint8_t *sc = q.scales + scale_at(r, b, kt);
-  const int k0 = b * BLK;
-  uint8_t *c = q.codes + r * code_pitch(q.k) + k0 / 2;
-  if (r >= q.rows || k0 >= q.k) {
-    *sc = 0;
-    // the second half of a 32-value group whose last block is missing
-    if (r < q.rows && (size_t)k0 / 2 < code_pitch(q.k))
-      for (int i = 0; i < BLK / 2; ++i) c[i] = 0;
-    return;
+// A lane takes 8 consecutive values of a row, a warp 256 (or, for short rows,
+// one scale tile's 64 or 128 of adjacent rows), and of each of the rows r, r + 32, r + 64, r + 96
+// whose scale words lie side by side in a scale tile, so that the scales go
+// out in 16-byte pieces and four loads are in flight per lane.  A block spans
+// two (NV) or four lanes; its largest magnitude and the tile's scale words are
+// joined by shuffles.
+constexpr int QT_WARPS = 8;
+
+// 8 values from x[k0 ..], zeros from k on; `vec`: rows are 16-byte aligned.
+template <int TY>
+T0B_DEV void load8(const typename Plain<TY>::T *x, int k0, int k, bool vec, float *v) {
+  using T = typename Plain<TY>::T;
+  if (vec && k0 + 8 <= k) {
+    uint4 t[sizeof(T) / 2];
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) t[i] = reinterpret_cast<const uint4 *>(x + k0)[i];
+    const T *e = reinterpret_cast<const T *>(t);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = Plain<TY>::get(e[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = k0 + i < k ? Plain<TY>::get(x[k0 + i]) : 0.0f;
   }
-  float v[BLK];
-  uint32_t amax = 0;
-  for (int i = 0; i < BLK; ++i) {
-    v[i] = k0 + i < q.k ? Plain<TY>::get(x[r * ldx + k0 + i]) : 0.0f;
-    amax = max(amax, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-  }
-  const BlockScale<NV> s(amax, q.ts);
-  *sc = (uint8_t)s.byte;
-  uint32_t w[BLK / 8];
-  quantize_block<NV>(s, v, w);
-  for (int i = 0; i < BLK / 2; ++i) c[i] = (uint8_t)(w[i / 4] >> (i % 4 * 8));
 }
 
+// LPR: lanes along a row, a scale tile's (8 or 16) or 32.
+template <int TY, bool NV, int LPR>
+__global__ void __launch_bounds__(32 * QT_WARPS) fp4_quantize_kernel(const typename Plain<TY>::T *x, int64_t ldx, Fp4Mat q, bool vec) {
+  constexpr int BLK = NV ? 16 : 32, LB = BLK / 8;  // lanes of a block
+  constexpr int RPW = 32 / LPR;                    // adjacent rows of a warp
+  const int kt = (q.k + 4 * BLK - 1) / (4 * BLK);
+  const int lane = threadIdx.x & 31;
+  const int r0 = blockIdx.x * (QT_WARPS * RPW) + (threadIdx.x >> 5) * RPW + lane / LPR;  // counts 32 rows of each group
+  const int group = r0 >> 5, r = group * 128 + (r0 & 31);
+  const int k0 = (blockIdx.y * LPR + lane % LPR) * 8;
+  pdl_wait();
+  pdl_launch_dependents();
+  float v[4][8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (r + 32 * i < q.rows)
+      load8<TY>(x + (r + 32 * i) * ldx, k0, q.k, vec, v[i]);
+    else
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[i][j] = 0.0f;
+  }
+  uint32_t sc[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t amax = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) amax = max(amax, __float_as_uint(v[i][j]) & 0x7FFFFFFFu);
+#pragma unroll
+    for (int o = 1; o < LB; o *= 2) amax = max(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, o));
+    const BlockScale<NV> s(amax, q.ts);
+    sc[i] = s.byte << (8 * (lane / LB % 4));
+    sc[i] |= __shfl_xor_sync(0xFFFFFFFFu, sc[i], LB);
+    sc[i] |= __shfl_xor_sync(0xFFFFFFFFu, sc[i], 2 * LB);
+    uint32_t w;
+    quantize8<NV>(s, v[i], &w);
+    if (r + 32 * i < q.rows && k0 / 2 < (int)code_pitch(q.k))
+      *reinterpret_cast<uint32_t *>(q.codes + (r + 32 * i) * code_pitch(q.k) + k0 / 2) = w;
+  }
+  const int t = k0 / (4 * BLK);
+  if (lane % (4 * LB) == 0 && t < kt && group < (q.rows + 127) / 128)
+    *reinterpret_cast<uint4 *>(q.scales + ((size_t)group * kt + t) * 512 + (r & 31) * 16) = make_uint4(sc[0], sc[1], sc[2], sc[3]);
+}
+
+// ----------------------------------------------------------- the other way
+// The same division of work: 4 bytes of codes to 8 values a lane, the scale
+// words of four rows in one 16-byte load.
 template <int TY>
-__global__ void fp4_dequantize_kernel(Fp4Mat q, typename Plain<TY>::T *y, int64_t ldy) {
-  const int kt = (q.k + 4 * q.blk - 1) / (4 * q.blk);
-  const size_t id = blockIdx.x * (size_t)blockDim.x + threadIdx.x;
-  const int64_t r = id / q.k;
-  const int k = (int)(id % q.k);
-  if (r >= q.rows) return;
-  const uint32_t c = q.codes[r * code_pitch(q.k) + k / 2] >> (k % 2 * 4) & 15;
-  const float s = scale_value(q.blk, q.scales[scale_at((int)r, k / q.blk, kt)]);
-  y[r * ldy + k] = Plain<TY>::put(code_value(c) * s * q.ts);
+T0B_DEV void store8(typename Plain<TY>::T *y, int k0, int k, bool vec, const float *v) {
+  using T = typename Plain<TY>::T;
+  alignas(16) T t[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) t[i] = Plain<TY>::put(v[i]);
+  if (vec && k0 + 8 <= k) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4 *>(y + k0)[i] = reinterpret_cast<const uint4 *>(t)[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (k0 + i < k) y[k0 + i] = t[i];
+  }
+}
+
+template <int TY, bool NV, int LPR>
+__global__ void __launch_bounds__(32 * QT_WARPS) fp4_dequantize_kernel(Fp4Mat q, typename Plain<TY>::T *y, int64_t ldy, bool vec) {
+  constexpr int BLK = NV ? 16 : 32, LB = BLK / 8, RPW = 32 / LPR;
+  const int kt = (q.k + 4 * BLK - 1) / (4 * BLK);
+  const int lane = threadIdx.x & 31;
+  const int r0 = blockIdx.x * (QT_WARPS * RPW) + (threadIdx.x >> 5) * RPW + lane / LPR;
+  const int group = r0 >> 5, r = group * 128 + (r0 & 31);
+  const int k0 = (blockIdx.y * LPR + lane % LPR) * 8;
+  pdl_wait();
+  pdl_launch_dependents();
+  if (k0 >= q.k || r >= q.rows) return;
+  const uint4 s4 = *reinterpret_cast<const uint4 *>(q.scales + ((size_t)group * kt + k0 / (4 * BLK)) * 512 + (r & 31) * 16);
+  const uint32_t sw[4] = {s4.x, s4.y, s4.z, s4.w};
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (r + 32 * i < q.rows) w[i] = *reinterpret_cast<const uint32_t *>(q.codes + (r + 32 * i) * code_pitch(q.k) + k0 / 2);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (r + 32 * i >= q.rows) break;
+    const float s = scale_value<NV>(sw[i] >> (8 * (lane / LB % 4)) & 255);
+    float v[8];
+    values8(w[i], v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = NV ? v[j] * s * q.ts : v[j] * s;
+    store8<TY>(y + (r + 32 * i) * ldy, k0, q.k, vec, v);
+  }
 }
 
 // ----------------------------------------------------------------- product
@@ -310,7 +388,8 @@ T0B_DEV void store_quant32(const Fp4Mat &q, int r, int c0, float *v) {
     for (int j = 0; j < BLK; ++j) amax = max(amax, __float_as_uint(v[b * BLK + j]) & 0x7FFFFFFFu);
     const BlockScale<NV> s(amax, q.ts);
     sc |= s.byte << (8 * b);
-    quantize_block<NV>(s, v + b * BLK, w + b * BLK / 8);
+#pragma unroll
+    for (int i = 0; i < BLK / 8; ++i) quantize8<NV>(s, v + b * BLK + 8 * i, w + b * BLK / 8 + i);
   }
   uint8_t *ps = q.scales + scale_at(r, c0 / BLK, kt);
   if (NV)
@@ -397,6 +476,8 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
   cluster_sync_all();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  pdl_wait();
+  pdl_launch_dependents();
   auto lead = [](const uint64_t *b) { return mapa_shared(smem_u32(b), 0); };
   // first weight row of this CTA's half, and of each half's scales
   auto w_row = [&](int nt, uint32_t half) { return GLU ? nt * 128 + (half ? p.up_row : 0) : nt * 256 + 128 * (int)half; };
@@ -404,7 +485,6 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
   if (warp == 0 && lane == 0) {
     // ------------------------------------------------------------ loads (both CTAs)
     uint32_t g = 0;
-    pdl_wait();
     for (int tile = pair; tile < p.n_tiles && !*abort_flag; tile += npairs) {
       const int nt = tile % p.n_tiles_n, m0 = tile / p.n_tiles_n * 256 + 128 * (int)rank;
       for (int s = 0; s < S && !*abort_flag; ++s, ++g) {
@@ -559,12 +639,26 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
 }
 
 // ------------------------------------------------------------- host side
+// Every kernel here starts while the previous one of the stream ends and
+// waits for it (griddepcontrol.wait) before its first access to memory that a
+// kernel may have written.
+cudaLaunchAttribute dependent_launch() {
+  cudaLaunchAttribute a{};
+  a.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  a.val.programmaticStreamSerializationAllowed = 1;
+  return a;
+}
+
 template <typename... P, typename... A>
 cudaError_t launch(void (*k)(P...), dim3 grid, dim3 block, cudaStream_t st, A... args) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid;
   cfg.blockDim = block;
   cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0] = dependent_launch();
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, k, args...);
 }
 
@@ -613,7 +707,8 @@ cudaError_t launch_pair(const Fp4Mat &w, const Fp4Mat &x, Fp4Args p, cudaStream_
   const int64_t tiles = (int64_t)p.n_tiles_n * ((p.M + 255) / 256);
   if (tiles > INT32_MAX / 2) return cudaErrorInvalidValue;
   p.n_tiles = (int)tiles;
-  cudaLaunchAttribute at[1];
+  cudaLaunchAttribute at[2];
+  at[1] = dependent_launch();
   at[0].id = cudaLaunchAttributeClusterDimension;
   at[0].val.clusterDim.x = 2;
   at[0].val.clusterDim.y = 1;
@@ -623,7 +718,7 @@ cudaError_t launch_pair(const Fp4Mat &w, const Fp4Mat &x, Fp4Args p, cudaStream_
   cfg.dynamicSmemBytes = C::SMEM;
   cfg.stream = st;
   cfg.attrs = at;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   const int pairs = max_pairs((const void *)kfn, cfg);
   if (pairs < 1) return cudaErrorInvalidConfiguration;
   cfg.gridDim = dim3(2 * (p.n_tiles < pairs ? p.n_tiles : pairs));
@@ -645,28 +740,39 @@ cudaError_t gemm_fmt(const Fp4Mat &w, const Fp4Mat &x, const Fp4Out &out, const 
   return gemm_ty<NV, TY_BF16>(w, x, out, p, st);
 }
 
-template <int TY>
-cudaError_t quantize_ty(const void *x, int64_t ldx, const Fp4Mat &q, cudaStream_t st) {
+bool rows_aligned(const void *p, int64_t ld, int type) { return ((uintptr_t)p | (uint64_t)ld * (type == TY_F32 ? 4 : 2)) % 16 == 0; }
+
+// Rows of one scale tile's width get the lanes of one tile, longer ones a warp.
+template <int TY, bool NV, bool QUANT>
+cudaError_t convert(const void *x, int64_t ld, const Fp4Mat &q, cudaStream_t st) {
   using T = typename Plain<TY>::T;
-  const size_t n = (size_t)((q.rows + 127) / 128 * 128) * ((q.k + 4 * q.blk - 1) / (4 * q.blk) * 4);
-  const dim3 grid((unsigned)((n + 127) / 128));
-  return q.blk == 16 ? launch(fp4_quantize_kernel<TY, true>, grid, 128, st, (const T *)x, ldx, q)
-                     : launch(fp4_quantize_kernel<TY, false>, grid, 128, st, (const T *)x, ldx, q);
+  constexpr int SHORT = NV ? 8 : 16;
+  const bool vec = rows_aligned(x, ld, TY), narrow = q.k <= 8 * SHORT;
+  const int lpr = narrow ? SHORT : 32, row_warps = (q.rows + 127) / 128 * lpr;  // of 32 / lpr rows, 32 rows a group
+  const int width = QUANT ? (q.k + 8 * SHORT - 1) / (8 * SHORT) * (8 * SHORT) : q.k;  // whole scale tiles
+  const dim3 grid((row_warps + QT_WARPS - 1) / QT_WARPS, (width + 8 * lpr - 1) / (8 * lpr));
+  if constexpr (QUANT)
+    return narrow ? launch(fp4_quantize_kernel<TY, NV, SHORT>, grid, 32 * QT_WARPS, st, (const T *)x, ld, q, vec)
+                  : launch(fp4_quantize_kernel<TY, NV, 32>, grid, 32 * QT_WARPS, st, (const T *)x, ld, q, vec);
+  else
+    return narrow ? launch(fp4_dequantize_kernel<TY, NV, SHORT>, grid, 32 * QT_WARPS, st, q, (T *)x, ld, vec)
+                  : launch(fp4_dequantize_kernel<TY, NV, 32>, grid, 32 * QT_WARPS, st, q, (T *)x, ld, vec);
+}
+template <bool NV, bool QUANT>
+cudaError_t convert_ty(int type, const void *x, int64_t ld, const Fp4Mat &q, cudaStream_t st) {
+  if (type == TY_F32) return convert<TY_F32, NV, QUANT>(x, ld, q, st);
+  if (type == TY_F16) return convert<TY_F16, NV, QUANT>(x, ld, q, st);
+  return convert<TY_BF16, NV, QUANT>(x, ld, q, st);
 }
 
 }  // namespace
 
 cudaError_t t0b_launch_fp4_quantize(int x_type, const void *x, int64_t ldx, const Fp4Mat &q, cudaStream_t st) {
-  if (x_type == TY_F32) return quantize_ty<TY_F32>(x, ldx, q, st);
-  if (x_type == TY_F16) return quantize_ty<TY_F16>(x, ldx, q, st);
-  return quantize_ty<TY_BF16>(x, ldx, q, st);
+  return q.blk == 16 ? convert_ty<true, true>(x_type, x, ldx, q, st) : convert_ty<false, true>(x_type, x, ldx, q, st);
 }
 
 cudaError_t t0b_launch_fp4_dequantize(const Fp4Mat &q, int y_type, void *y, int64_t ldy, cudaStream_t st) {
-  const dim3 grid((unsigned)(((size_t)q.rows * q.k + 127) / 128));
-  if (y_type == TY_F32) return launch(fp4_dequantize_kernel<TY_F32>, grid, 128, st, q, (float *)y, ldy);
-  if (y_type == TY_F16) return launch(fp4_dequantize_kernel<TY_F16>, grid, 128, st, q, (__half *)y, ldy);
-  return launch(fp4_dequantize_kernel<TY_BF16>, grid, 128, st, q, (__nv_bfloat16 *)y, ldy);
+  return q.blk == 16 ? convert_ty<true, false>(y_type, y, ldy, q, st) : convert_ty<false, false>(y_type, y, ldy, q, st);
 }
 
 cudaError_t t0b_launch_fp4_gemm(const Fp4Mat &w, const Fp4Mat &x, const Fp4Out &out, int *err, cudaStream_t st) {
@@ -682,7 +788,6 @@ cudaError_t t0b_launch_fp4_gemm(const Fp4Mat &w, const Fp4Mat &x, const Fp4Out &
   p.q = out.q;
   p.up_row = out.glu ? p.n : 0;
   p.err = err;
-  const int es = out.type == TY_F32 ? 4 : 2;
-  p.vec = !out.quant && (uintptr_t)out.y % 16 == 0 && out.ld * es % 16 == 0;
+  p.vec = !out.quant && rows_aligned(out.y, out.ld, out.type);
   return w.blk == 16 ? gemm_fmt<true>(w, x, out, p, st) : gemm_fmt<false>(w, x, out, p, st);
 }
