@@ -81,6 +81,12 @@ T0B_DEV void values8(uint32_t w, float *v) {
   }
 }
 
+// max(a, |b|) that keeps a NaN (as bits above infinity's).
+T0B_DEV float absmax(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(fabsf(b)));
+  return r;
+}
 // A block's scale byte and the factors that divide by its scale, from the bits
 // of its largest magnitude (infinities and NaNs compare above every finite
 // value).  The quotients are correctly rounded, so that every rounding to 4
@@ -182,9 +188,10 @@ __global__ void __launch_bounds__(32 * QT_WARPS) fp4_quantize_kernel(const typen
   uint32_t sc[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    uint32_t amax = 0;
+    float top = 0.0f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) amax = max(amax, __float_as_uint(v[i][j]) & 0x7FFFFFFFu);
+    for (int j = 0; j < 8; ++j) top = absmax(top, v[i][j]);
+    uint32_t amax = __float_as_uint(top);
 #pragma unroll
     for (int o = 1; o < LB; o *= 2) amax = max(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, o));
     const BlockScale<NV> s(amax, q.ts);
@@ -333,6 +340,16 @@ T0B_DEV void umma_fp4_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, u
         : "memory");
 }
 
+// One lane of a converged warp, known to the compiler as such: what it issues
+// keeps its operands in uniform registers.  (Chosen by `lane == 0`, the MMA
+// warp issued an 8192 x 8192 x 8192 product's instructions in 360 us instead
+// of 193.)
+T0B_DEV bool elect_one() {
+  uint32_t ok;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xFFFFFFFF;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(ok));
+  return ok != 0;
+}
+
 // Arguments of the product kernels beside the tensor maps.
 struct Fp4Args {
   int M, n, K;     // tokens, result columns (a gated product's F), values
@@ -353,8 +370,12 @@ struct Fp4Args {
 // tiles of codes per step; CTA r holds tokens 128 r .. of the tile and weight
 // rows 128 r .. (gated: CTA 0 gate rows, CTA 1 the matching up rows), and the
 // scales of its tokens and of all 256 weight rows.
-constexpr int PAIR_EPI_WARPS = 8;
+constexpr int PAIR_EPI_WARPS = 16;
 constexpr int PAIR_THREADS = 128 + 32 * PAIR_EPI_WARPS;
+// Registers per thread (setmaxnreg): the kernel is launched with PAIR_REGS and
+// its warpgroups divide them; the host refuses a build with another count.
+constexpr int PAIR_REGS = 96, PAIR_REGS_LOW = 32, PAIR_REGS_EPI = 112;
+static_assert(PAIR_REGS_LOW * 128 + PAIR_REGS_EPI * 32 * PAIR_EPI_WARPS <= PAIR_REGS * PAIR_THREADS, "registers over the launch's");
 
 template <bool NV, bool ROT>
 struct PairCfg {
@@ -362,9 +383,11 @@ struct PairCfg {
   static constexpr uint32_t CODES = 128 * 128;             // one operand's codes of a stage
   static constexpr uint32_t SC = AT * 512;                 // 128 rows' scales of a stage
   static constexpr uint32_t STAGE = 2 * CODES + (ROT ? 5 : 3) * SC;
-  static constexpr int NS = 5;                             // stages
+  static constexpr int NS = NV && ROT ? 4 : 5;             // stages
   static constexpr uint32_t OFF_A = 0, OFF_B = CODES, OFF_SA = 2 * CODES, OFF_SB = OFF_SA + SC, OFF_RAW = OFF_SB + 2 * SC;
-  static constexpr uint32_t OFF_BIAS = NS * STAGE, OFF_BAR = OFF_BIAS + 256 * 4, SMEM = OFF_BAR + 256 + 1024;
+  static constexpr uint32_t OFF_STG = NS * STAGE;          // 32 rows x 64 bytes per epilogue warp
+  static constexpr uint32_t OFF_BIAS = OFF_STG + PAIR_EPI_WARPS * 2048, OFF_BAR = OFF_BIAS + 256 * 4;
+  static constexpr uint32_t SMEM = OFF_BAR + 256 + 1024;
   static constexpr uint32_t SFC = AT * 12;                 // TMEM columns of a stage's scales
   static_assert(256 + NS * SFC <= 512, "accumulator and scales in TMEM");
   static_assert(STAGE % 1024 == 0 && SMEM <= 232448, "shared memory");
@@ -377,15 +400,18 @@ T0B_DEV void store_quant32(const Fp4Mat &q, int r, int c0, float *v) {
   constexpr int BLK = NV ? 16 : 32, NB = 32 / BLK;
   const int kt = (q.k + 4 * BLK - 1) / (4 * BLK);
   if (r >= (q.rows + 127) / 128 * 128 || c0 >= kt * 4 * BLK) return;
+  if (r >= q.rows || c0 + 32 > q.k) {
 #pragma unroll
-  for (int j = 0; j < 32; ++j)
-    if (r >= q.rows || c0 + j >= q.k) v[j] = 0.0f;
+    for (int j = 0; j < 32; ++j)
+      if (r >= q.rows || c0 + j >= q.k) v[j] = 0.0f;
+  }
   uint32_t w[4], sc = 0;
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
-    uint32_t amax = 0;
+    float top = 0.0f;
 #pragma unroll
-    for (int j = 0; j < BLK; ++j) amax = max(amax, __float_as_uint(v[b * BLK + j]) & 0x7FFFFFFFu);
+    for (int j = 0; j < BLK; ++j) top = absmax(top, v[b * BLK + j]);
+    const uint32_t amax = __float_as_uint(top);
     const BlockScale<NV> s(amax, q.ts);
     sc |= s.byte << (8 * b);
 #pragma unroll
@@ -399,24 +425,42 @@ T0B_DEV void store_quant32(const Fp4Mat &q, int r, int c0, float *v) {
   if (r < q.rows && c0 < q.k) *reinterpret_cast<uint4 *>(q.codes + r * code_pitch(q.k) + c0 / 2) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// Writes 32 consecutive values of one row, columns c0 .. of n.
+// 32 rows x 64 bytes of the result, one row per lane, columns c0 .. : through
+// the warp's staging buffer (64-byte swizzle) and out by a TMA store, or, where
+// the result's rows are not 16-byte aligned, element by element along the rows.
 template <int TY>
-T0B_DEV void store_row32(const Fp4Args &p, int m, int c0, const float *v) {
+T0B_DEV void store_rows(const Fp4Args &p, const void *tm_y, uint8_t *stg, int row0, int c0, const float *v) {
   using T = typename Plain<TY>::T;
-  T *dst = reinterpret_cast<T *>(p.y) + m * p.ld + c0;
-  if (p.vec && c0 + 32 <= p.n) {
+  constexpr int W = 64 / sizeof(T);
+  const int lane = threadIdx.x & 31;
+  if (p.vec) {
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+  }
+  __syncwarp();  // the buffer has been read
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
     constexpr int PER = 16 / sizeof(T);
+    alignas(16) T t[PER];
 #pragma unroll
-    for (int i = 0; i < 32 / PER; ++i) {
-      alignas(16) T t[PER];
-#pragma unroll
-      for (int j = 0; j < PER; ++j) t[j] = Plain<TY>::put(v[i * PER + j]);
-      reinterpret_cast<uint4 *>(dst)[i] = *reinterpret_cast<const uint4 *>(t);
+    for (int j = 0; j < PER; ++j) t[j] = Plain<TY>::put(v[i * PER + j]);
+    *reinterpret_cast<uint4 *>(stg + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4)) = *reinterpret_cast<const uint4 *>(t);
+  }
+  if (p.vec) {
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      if (row0 < p.M && c0 < p.n) tma_store_2d(tm_y, stg, c0, row0);
+      bulk_commit();
     }
   } else {
-#pragma unroll
-    for (int j = 0; j < 32; ++j)
-      if (c0 + j < p.n) dst[j] = Plain<TY>::put(v[j]);
+    __syncwarp();
+    T *y = reinterpret_cast<T *>(p.y);
+    const int c = lane % W;
+#pragma unroll 4
+    for (int r = lane / W; r < 32; r += 32 / W)
+      if (row0 + r < p.M && c0 + c < p.n)
+        y[(row0 + r) * p.ld + c0 + c] =
+            *reinterpret_cast<const T *>(stg + r * 64 + (((c * (int)sizeof(T) >> 4) ^ ((r >> 1) & 3)) << 4) + (c * (int)sizeof(T) & 15));
   }
 }
 
@@ -424,7 +468,8 @@ T0B_DEV void store_row32(const Fp4Args &p, int m, int c0, const float *v) {
 template <bool NV, bool GLU, bool ROT, int TY>
 __global__ void __launch_bounds__(PAIR_THREADS, 1)
     fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
-                         const __grid_constant__ CUtensorMap tm_xs, const __grid_constant__ CUtensorMap tm_ws, Fp4Args p) {
+                         const __grid_constant__ CUtensorMap tm_xs, const __grid_constant__ CUtensorMap tm_ws,
+                         const __grid_constant__ CUtensorMap tm_y, Fp4Args p) {
   using C = PairCfg<NV, ROT>;
   constexpr int AT = C::AT, NS = C::NS;
   extern __shared__ uint8_t smem_raw[];
@@ -445,7 +490,7 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(mma_done + 1);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(mma_done + 2);
   float *sbias = reinterpret_cast<float *>(smem + C::OFF_BIAS);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int S = (p.K + 255) / 256;
   const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
 
@@ -482,7 +527,9 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
   // first weight row of this CTA's half, and of each half's scales
   auto w_row = [&](int nt, uint32_t half) { return GLU ? nt * 128 + (half ? p.up_row : 0) : nt * 256 + 128 * (int)half; };
 
-  if (warp == 0 && lane == 0) {
+  if (warp < 4) {
+  setmaxnreg_dec<PAIR_REGS_LOW>();
+  if (warp == 0 && elect_one()) {
     // ------------------------------------------------------------ loads (both CTAs)
     uint32_t g = 0;
     for (int tile = pair; tile < p.n_tiles && !*abort_flag; tile += npairs) {
@@ -508,7 +555,7 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
         }
       }
     }
-  } else if (warp == 1 && lane == 0 && rank == 0) {
+  } else if (warp == 1 && rank == 0 && elect_one()) {
     // ------------------------------------------------------------ MMA (CTA 0)
     constexpr uint32_t idesc = idesc_fp4<NV>(256, 256);
     uint32_t g = 0, it = 0;
@@ -573,61 +620,64 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
         if (lane == 0) mbar_arrive_cluster(lead(&rot_full[sl]));
       }
     }
-  } else if (warp >= 4) {
+  }
+  } else {
     // ------------------------------------------------------------ epilogue (both CTAs)
-    const int q = warp & 3, h = (warp - 4) >> 2;  // lane quarter, column half
+    setmaxnreg_inc<PAIR_REGS_EPI>();
+    const int q = warp & 3, h = (warp - 4) >> 2;  // lane quarter, 64 columns (gated: 32 gate, 32 up)
     const int et = threadIdx.x - 128;
+    uint8_t *stg = smem + C::OFF_STG + (warp - 4) * 2048;
     uint32_t it = 0;
     for (int tile = pair; tile < p.n_tiles; tile += npairs, ++it) {
       const int nt = tile % p.n_tiles_n, m0 = tile / p.n_tiles_n * 256 + 128 * (int)rank;
-      asm volatile("bar.sync 1, 256;" ::: "memory");
-      {
+      asm volatile("bar.sync 1, 512;" ::: "memory");
+      if (et < 256) {
         const int col = GLU ? nt * 128 + (et & 127) : nt * 256 + et;
         sbias[et] = p.bias && col < p.n ? p.bias[GLU && et >= 128 ? p.n + col : col] : 0.0f;
       }
-      asm volatile("bar.sync 1, 256;" ::: "memory");
-      const int m = m0 + 32 * q + lane;
+      asm volatile("bar.sync 1, 512;" ::: "memory");
+      const int row0 = m0 + 32 * q;
       const uint32_t trow = tmem + ((uint32_t)(32 * q) << 16);
       bool have = mbar_wait(acc_full, it & 1, p.err, T0B_DEVERR_WAIT_ACC, abort_flag) && !*abort_flag;
       have = __all_sync(0xFFFFFFFFu, have);
       tc_fence_after();
-      uint32_t r[4][32];  // 128 columns (gated: 64 gate, 64 up)
+      uint32_t r[2][32];
       if (have) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) tmem_ld32(trow + (GLU ? 64 * h + 128 * (i >> 1) + 32 * (i & 1) : 128 * h + 32 * i), r[i]);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) tmem_ld_wait(r[i]);
+        tmem_ld32(trow + (GLU ? 32 : 64) * h, r[0]);
+        tmem_ld32(trow + (GLU ? 128 + 32 * h : 64 * h + 32), r[1]);
+        tmem_ld_wait(r[0]);
+        tmem_ld_wait(r[1]);
       }
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(lead(acc_empty));
       if (!have) continue;
+      constexpr int OT = TY < 0 ? TY_F32 : TY, W = OT == TY_F32 ? 16 : 32;
       if constexpr (!GLU) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int c0 = 128 * h + 32 * i;
-          float *v = reinterpret_cast<float *>(r[i]);
+        for (int i = 0; i < 64 / W; ++i) {
+          const int c0 = 64 * h + W * i;
+          float v[W];
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = fmaf(__uint_as_float(r[i][j]), p.alpha, sbias[c0 + j]);
-          if (m < p.M && nt * 256 + c0 < p.n) store_row32<TY < 0 ? TY_F32 : TY>(p, m, nt * 256 + c0, v);
+          for (int j = 0; j < W; ++j) v[j] = fmaf(__uint_as_float(r[i * W / 32][i * W % 32 + j]), p.alpha, sbias[c0 + j]);
+          store_rows<OT>(p, &tm_y, stg, row0, nt * 256 + c0, v);
         }
       } else {
+        const int c0 = 32 * h, f0 = nt * 128 + c0;
+        float v[32];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int c0 = 64 * h + 32 * i, f0 = nt * 128 + c0;
-          float v[32];
+        for (int j = 0; j < 32; ++j)
+          v[j] = silu_mul(fmaf(__uint_as_float(r[0][j]), p.alpha, sbias[c0 + j]),
+                          fmaf(__uint_as_float(r[1][j]), p.alpha, sbias[128 + c0 + j]));
+        if constexpr (TY >= 0) {
 #pragma unroll
-          for (int j = 0; j < 32; ++j)
-            v[j] = silu_mul(fmaf(__uint_as_float(r[i][j]), p.alpha, sbias[c0 + j]),
-                            fmaf(__uint_as_float(r[2 + i][j]), p.alpha, sbias[128 + c0 + j]));
-          if constexpr (TY >= 0) {
-            if (m < p.M && f0 < p.n) store_row32<TY < 0 ? TY_F32 : TY>(p, m, f0, v);
-          } else {
-            store_quant32<NV>(p.q, m, f0, v);
-          }
+          for (int i = 0; i < 32 / W; ++i) store_rows<OT>(p, &tm_y, stg, row0, f0 + W * i, v + W * i);
+        } else {
+          store_quant32<NV>(p.q, row0 + lane, f0, v);
         }
       }
     }
+    if (lane == 0) bulk_wait_all();
   }
   tc_fence_before();
   __syncthreads();
@@ -698,10 +748,18 @@ template <bool NV, bool GLU, bool ROT, int TY>
 cudaError_t launch_pair(const Fp4Mat &w, const Fp4Mat &x, Fp4Args p, cudaStream_t st) {
   using C = PairCfg<NV, ROT>;
   auto kfn = fp4_gemm_pair_kernel<NV, GLU, ROT, TY>;
+  static const int regs = [&] {
+    cudaFuncAttributes fa{};
+    return cudaFuncGetAttributes(&fa, (const void *)kfn) == cudaSuccess ? fa.numRegs : -1;
+  }();
+  if (regs != PAIR_REGS) return cudaErrorInvalidConfiguration;
   cudaError_t e = t0b_smem_limit((const void *)kfn, C::SMEM);
   if (e != cudaSuccess) return e;
   CUtensorMap tx, tw, txs, tws;
   if (!code_map(&tx, x) || !code_map(&tw, w) || !scale_map(&txs, x, p.kt, C::AT) || !scale_map(&tws, w, p.kt, C::AT))
+    return cudaErrorInvalidValue;
+  CUtensorMap ty = tx;  // not used without aligned rows
+  if (p.vec && !t0b_make_tmap_rows64(&ty, p.y, TY == TY_F32 ? 4 : 2, (uint64_t)p.n, (uint64_t)p.M, (uint64_t)p.ld))
     return cudaErrorInvalidValue;
   p.n_tiles_n = GLU ? (p.n + 127) / 128 : (p.n + 255) / 256;
   const int64_t tiles = (int64_t)p.n_tiles_n * ((p.M + 255) / 256);
@@ -722,7 +780,7 @@ cudaError_t launch_pair(const Fp4Mat &w, const Fp4Mat &x, Fp4Args p, cudaStream_
   const int pairs = max_pairs((const void *)kfn, cfg);
   if (pairs < 1) return cudaErrorInvalidConfiguration;
   cfg.gridDim = dim3(2 * (p.n_tiles < pairs ? p.n_tiles : pairs));
-  return cudaLaunchKernelEx(&cfg, kfn, tx, tw, txs, tws, p);
+  return cudaLaunchKernelEx(&cfg, kfn, tx, tw, txs, tws, ty, p);
 }
 
 template <bool NV, int TY>

@@ -873,6 +873,13 @@ bool t0b_make_tmap_u8_2d(CUtensorMap *tm, const void *ptr, uint64_t inner, uint6
                       CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
+// Tensor [outer][inner] of 2- or 4-byte elements, rows ld elements apart, box
+// of 32 rows x 64 bytes with the 64-byte swizzle: the 4-bit products' results.
+bool t0b_make_tmap_rows64(CUtensorMap *tm, const void *ptr, int elem, uint64_t inner, uint64_t outer, uint64_t ld) {
+  return make_tmap_2d(tm, elem == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, ptr, inner, outer,
+                      ld * elem, 64 / elem, 32, CU_TENSOR_MAP_SWIZZLE_64B);
+}
+
 // f16 tensor of dims {d0, d1, d2} (innermost first; d1 rows s1 bytes apart,
 // d2 slabs s2 bytes apart), box {b0, b1, b2}, optionally with the 128-byte
 // swizzle: for the attention kernels' TMA stores.
