@@ -688,6 +688,382 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
   }
 }
 
+// ------------------------------------------------- product, few tokens
+// The product for launches with few pair tiles: a CTA multiplies 128 weight
+// rows (MMA rows; gated: 128 gate rows and the 128 matching up rows, two
+// accumulators) with up to 128 tokens (MMA columns) over one slice of K, and
+// the slices of a tile form a thread-block cluster.  Every SM gets a share of
+// the weights, which is what such a product has to read; the partial tiles
+// meet in distributed shared memory, each CTA adding the slices of its share
+// of the tokens in slice order.  With rows as lanes the results of a token are
+// 32 consecutive columns of a warp: stores are coalesced whatever the row
+// stride, and a 4-bit result's blocks are joined by shuffles.  FUSED: x is
+// plain and each CTA quantises its slice of the tokens into shared memory
+// itself (one launch, no 4-bit activations in memory).
+constexpr int SPLIT_THREADS = 256;
+constexpr int SPLIT_MAX_NS = 6, SPLIT_MAX_CLUSTER = 8;
+
+struct SplitArgs {
+  Fp4Args a;
+  int NT, CS, SL, NS;       // tokens of a tile (a multiple of 8), K slices, stages of a slice, ring depth
+  int rt;                   // weight row tiles
+  uint32_t stage;           // bytes of a ring stage
+  uint32_t off_x, off_xs;   // FUSED: the slice's activation codes and scales
+  uint32_t off_slot, off_bar;
+  uint32_t tmem_cols;
+  int out_type;             // ggml type of y, or -1: the 4-bit result
+  int rot;                  // gated: up rows' scales must be moved (F % 128 != 0)
+  int early;                // the previous kernel on the stream does not write the weights
+  const void *x;            // FUSED
+  int x_type;
+  int64_t ldx;
+  float x_ts;
+  int xvec;
+};
+
+T0B_DEV void store_elem(void *y, int type, int64_t i, float v) {
+  if (type == TY_F32)
+    reinterpret_cast<float *>(y)[i] = v;
+  else if (type == TY_F16)
+    reinterpret_cast<__half *>(y)[i] = __float2half_rn(v);
+  else
+    reinterpret_cast<__nv_bfloat16 *>(y)[i] = __float2bfloat16_rn(v);
+}
+
+// One value per lane, 32 consecutive columns c0 .. c0 + 31 of row r (zeros
+// behind the matrix) to 4 bits.  Every lane of the warp calls it; c0 is a
+// multiple of 32.  Rows behind the matrix get zero scales.
+template <bool NV>
+T0B_DEV void quantize_lanes(const Fp4Mat &q, int r, int c0, float v) {
+  constexpr int BLK = NV ? 16 : 32;
+  const int lane = threadIdx.x & 31, kt = (q.k + 4 * BLK - 1) / (4 * BLK);
+  float top = absmax(0.0f, v);
+#pragma unroll
+  for (int o = BLK / 2; o; o >>= 1) top = absmax(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+  const BlockScale<NV> s(__float_as_uint(top), q.ts);
+  // eight lanes' values to every eighth lane
+  float u[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) u[j] = __shfl_sync(0xFFFFFFFFu, v, (lane & 24) + j);
+  uint32_t w;
+  quantize8<NV>(s, u, &w);
+  const int b = (c0 + lane) / BLK;
+  if (lane % BLK == 0 && b < 4 * kt) q.scales[scale_at(r, b, kt)] = r < q.rows && b * BLK < q.k ? (uint8_t)s.byte : 0;
+  if (lane % 8 == 0 && r < q.rows && (c0 + lane) / 2 < (int)code_pitch(q.k))
+    *reinterpret_cast<uint32_t *>(q.codes + r * code_pitch(q.k) + (c0 + lane) / 2) = w;
+}
+
+T0B_DEV void tmem_ld8(uint32_t addr, float *v) {
+  uint32_t r[8];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+      : "r"(addr)
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[i]);
+}
+T0B_DEV void scale_cp(uint32_t taddr, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+template <bool NV>
+T0B_DEV void umma_fp4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t acc) {
+  if constexpr (NV)
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %6, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(acc)
+        : "memory");
+  else
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %6, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(acc)
+        : "memory");
+}
+T0B_DEV void umma_commit(uint64_t *bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+T0B_DEV void st_cluster_f32(uint32_t addr, float v) {
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
+}
+
+// Bytes of a stage: weight codes, weight scales (gated: two halves, and room
+// for the up rows' scales as they are held), then, unless FUSED, the tokens'.
+template <bool NV, bool GLU, bool FUSED>
+__host__ __device__ constexpr uint32_t split_stage(int NT) {
+  const uint32_t sc = (NV ? 4 : 2) * 512;
+  const uint32_t n = (GLU ? 2 : 1) * 16384u + (GLU ? 4 : 1) * sc + (FUSED ? 0u : (uint32_t)NT * 128u + sc);
+  return (n + 1023u) & ~1023u;
+}
+
+template <int TY, bool NV>
+T0B_DEV void quantize_slice(const SplitArgs &p, uint8_t *codes, uint8_t *scales, int m0, int toks, int k_begin, int stages) {
+  // a warp takes 256 values (a stage) of a token; four at a time
+  constexpr int AT = NV ? 4 : 2, BLK = NV ? 16 : 32, LB = BLK / 8, U = 4;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const auto *x = reinterpret_cast<const typename Plain<TY>::T *>(p.x);
+  const int n = toks * stages;
+  for (int i0 = warp; i0 < n; i0 += U * (SPLIT_THREADS / 32)) {
+    float v[U][8];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * (SPLIT_THREADS / 32);
+      if (i < n) load8<TY>(x + (int64_t)(m0 + i / stages) * p.ldx, k_begin + i % stages * 256 + lane * 8, p.a.K, p.xvec, v[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * (SPLIT_THREADS / 32);
+      if (i >= n) break;
+      const int t = i / stages, s = i % stages;
+      float top = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) top = absmax(top, v[u][j]);
+#pragma unroll
+      for (int o = 1; o < LB; o *= 2) top = absmax(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+      const BlockScale<NV> sc(__float_as_uint(top), p.x_ts);
+      uint32_t w;
+      quantize8<NV>(sc, v[u], &w);
+      // 128-byte rows, 16-byte pieces swizzled by the row
+      *reinterpret_cast<uint32_t *>(codes + (size_t)s * p.NT * 128 + t * 128 + (((lane >> 2) ^ (t & 7)) << 4) + (lane & 3) * 4) = w;
+      if (lane % LB == 0)
+        scales[(s * AT + lane / (4 * LB)) * 512 + (t & 31) * 16 + (t >> 5) * 4 + lane / LB % 4] =
+            k_begin + s * 256 + lane * 8 < p.a.K ? (uint8_t)sc.byte : 0;
+    }
+  }
+}
+
+template <bool NV, bool GLU, bool FUSED>
+__global__ void __launch_bounds__(SPLIT_THREADS, 1)
+    fp4_gemm_split_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
+                          const __grid_constant__ CUtensorMap tm_xs, const __grid_constant__ CUtensorMap tm_ws, SplitArgs p) {
+  constexpr int AT = NV ? 4 : 2, H = GLU ? 2 : 1;
+  constexpr uint32_t SC = AT * 512, OFF_WS = H * 16384, OFF_RAW = OFF_WS + 2 * SC, OFF_X = OFF_WS + (GLU ? 4 : 1) * SC;
+  constexpr uint32_t SFC = AT * 4 * (H + 1);  // TMEM columns of a stage's scales
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t *smem = smem_raw + (base - smem_u32(smem_raw));
+  const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const int NT = p.NT, CS = p.CS, NS = p.NS;
+  if ((int)cluster_size() != CS) {
+    if (threadIdx.x == 0) record_error(p.a.err, T0B_DEVERR_SHAPE);
+    return;
+  }
+  const uint32_t OFF_XS = OFF_X + NT * 128;
+  uint64_t *full = reinterpret_cast<uint64_t *>(smem + p.off_bar), *empty = full + SPLIT_MAX_NS, *raw_full = empty + SPLIT_MAX_NS;
+  uint64_t *rot_full = raw_full + SPLIT_MAX_NS, *acc_full = rot_full + SPLIT_MAX_NS;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(acc_full + 1);
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(acc_full + 2);
+  const int rank = blockIdx.x % CS, tile = blockIdx.x / CS;
+  const int n0 = tile % p.rt * 128, m0 = tile / p.rt * NT;
+  const int toks = min(NT, p.a.M - m0);
+  const int S = (p.a.K + 255) / 256, s0 = rank * p.SL, ns = min(p.SL, S - s0);  // the host leaves no slice empty
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < SPLIT_MAX_NS; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+      mbar_init(&raw_full[i], 1);
+      mbar_init(&rot_full[i], 1);
+    }
+    mbar_init(acc_full, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+    fence_proxy_async_smem();
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(p.tmem_cols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (CS > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // running: its shared memory may be written
+  const uint32_t tmem = *tmem_slot;
+
+  auto load_w = [&](int i) {  // stage i of the slice
+    const int sl = i % NS, s = s0 + i;
+    uint8_t *st = smem + sl * p.stage;
+    const bool rot = GLU && p.rot;
+    mbar_arrive_expect_tx(&full[sl], H * 16384u + (GLU && !rot ? 2 : 1) * SC + (FUSED ? 0u : (uint32_t)NT * 128u + SC));
+    tma_load_2d(st, &tm_w, &full[sl], s * 128, n0);
+    tma_load_3d(st + OFF_WS, &tm_ws, &full[sl], 0, s * AT, n0 >> 7);
+    if constexpr (GLU) {
+      const int u0 = p.a.up_row + n0;
+      tma_load_2d(st + 16384, &tm_w, &full[sl], s * 128, u0);
+      if (!rot) {
+        tma_load_3d(st + OFF_WS + SC, &tm_ws, &full[sl], 0, s * AT, u0 >> 7);
+      } else {
+        mbar_arrive_expect_tx(&raw_full[sl], 2 * SC);
+        tma_load_3d(st + OFF_RAW, &tm_ws, &raw_full[sl], 0, s * AT, u0 >> 7);
+        tma_load_3d(st + OFF_RAW + SC, &tm_ws, &raw_full[sl], 0, s * AT, (u0 >> 7) + 1);
+      }
+    }
+  };
+  auto load_x = [&](int i) {
+    const int sl = i % NS, s = s0 + i;
+    uint8_t *st = smem + sl * p.stage;
+    tma_load_2d(st + OFF_X, &tm_x, &full[sl], s * 128, m0);
+    tma_load_3d(st + OFF_XS, &tm_xs, &full[sl], 0, s * AT, m0 >> 7);
+  };
+  const int first = min(ns, NS);
+  const bool loader = warp == 0 && elect_one();
+  if (loader && p.early)
+    for (int i = 0; i < first; ++i) load_w(i);
+  pdl_wait();
+  pdl_launch_dependents();
+  if (loader) {
+    if (!p.early)
+      for (int i = 0; i < first; ++i) load_w(i);
+    if constexpr (!FUSED)
+      for (int i = 0; i < first; ++i) load_x(i);
+  }
+  if constexpr (FUSED) {
+    __syncwarp();
+    uint8_t *xc = smem + p.off_x, *xs = smem + p.off_xs;
+    if (p.x_type == TY_F32)
+      quantize_slice<TY_F32, NV>(p, xc, xs, m0, toks, s0 * 256, ns);
+    else if (p.x_type == TY_F16)
+      quantize_slice<TY_F16, NV>(p, xc, xs, m0, toks, s0 * 256, ns);
+    else
+      quantize_slice<TY_BF16, NV>(p, xc, xs, m0, toks, s0 * 256, ns);
+    fence_proxy_async_smem();
+    __syncthreads();
+  }
+  if (loader) {
+    for (int i = first; i < ns; ++i) {
+      if (!mbar_wait(&empty[i % NS], (i / NS - 1) & 1, p.a.err, T0B_DEVERR_WAIT_EMPTY, abort_flag)) break;
+      load_w(i);
+      if constexpr (!FUSED) load_x(i);
+    }
+  } else if (warp == 1 && elect_one()) {
+    // ------------------------------------------------------------ MMA
+    const uint32_t idesc = idesc_fp4<NV>(128, 0) | (uint32_t)(NT >> 3) << 17;
+    const int steps = (p.a.K + 63) / 64;
+    const uint32_t sf_col = (uint32_t)(m0 & 127) >> 5;  // the tile's first token in its row group's scale columns
+    for (int i = 0; i < ns; ++i) {
+      const int sl = i % NS;
+      if (!mbar_wait(&full[sl], (i / NS) & 1, p.a.err, T0B_DEVERR_WAIT_X, abort_flag)) break;
+      if (GLU && p.rot && !mbar_wait(&rot_full[sl], (i / NS) & 1, p.a.err, T0B_DEVERR_WAIT_DEQ, abort_flag)) break;
+      tc_fence_after();
+      const uint32_t st = base + sl * p.stage, sf = tmem + H * NT + sl * SFC;
+      const uint32_t xc = FUSED ? base + p.off_x + i * NT * 128 : st + OFF_X;
+      const uint32_t xs = FUSED ? base + p.off_xs + i * SC : st + OFF_XS;
+#pragma unroll
+      for (int a = 0; a < AT; ++a) {
+        scale_cp(sf + 4 * a, scale_desc(xs + 512 * a));
+#pragma unroll
+        for (int h = 0; h < H; ++h) scale_cp(sf + 4 * AT * (1 + h) + 4 * a, scale_desc(st + OFF_WS + h * SC + 512 * a));
+      }
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk) {
+        if (4 * (s0 + i) + kk >= steps) break;
+        const int a = NV ? kk : kk / 2;
+#pragma unroll
+        for (int h = 0; h < H; ++h)
+          umma_fp4<NV>(tmem + h * NT, sw128_desc(st + h * 16384 + 32 * kk), sw128_desc(xc + 32 * kk),
+                       idesc | (NV ? 0u : idesc_scale_id(kk % 2 * 2)), sf + 4 * AT * (1 + h) + 4 * a,
+                       sf + 4 * a + sf_col, i > 0 || kk > 0);
+      }
+      umma_commit(&empty[sl]);
+    }
+    umma_commit(acc_full);  // also after a wait that ran out: what was issued completes before TMEM is given back
+  } else if (GLU && warp == 2 && p.rot) {
+    const int off = p.a.up_row & 127;
+    for (int i = 0; i < ns; ++i) {
+      const int sl = i % NS;
+      bool got = true;
+      if (lane == 0) got = mbar_wait(&raw_full[sl], (i / NS) & 1, p.a.err, T0B_DEVERR_WAIT_W, abort_flag);
+      if (!__shfl_sync(0xFFFFFFFFu, got ? 1 : 0, 0)) break;
+      const uint32_t *raw = reinterpret_cast<const uint32_t *>(smem + sl * p.stage + OFF_RAW);
+      uint32_t *dst = reinterpret_cast<uint32_t *>(smem + sl * p.stage + OFF_WS + SC);
+#pragma unroll
+      for (int a = 0; a < AT; ++a)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int r = off + 32 * j + lane;
+          dst[a * 128 + lane * 4 + j] = raw[(r >> 7) * (AT * 128) + a * 128 + (r & 31) * 4 + ((r >> 5) & 3)];
+        }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&rot_full[sl]);
+    }
+  }
+  __syncwarp();
+  if (CS > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+
+  // ------------------------------------------------------------ results
+  const int row = 32 * (warp & 3) + lane, n = n0 + row;  // warps 4 .. 7: this thread's weight row
+  const int share = (NT + CS - 1) / CS;                  // tokens whose slices this CTA adds
+  const uint32_t trow = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
+  bool have = true;
+  float b0 = 0.0f, b1 = 0.0f;
+  auto finish = [&](int t, float g, float u) {  // token t of the tile
+    const int m = m0 + t;
+    float v = fmaf(g, p.a.alpha, b0);
+    if constexpr (GLU) v = silu_mul(v, fmaf(u, p.a.alpha, b1));
+    if (p.out_type >= 0) {
+      if (n < p.a.n && m < p.a.M) store_elem(p.a.y, p.out_type, m * p.a.ld + n, v);
+    } else if constexpr (GLU) {
+      quantize_lanes<NV>(p.a.q, m, n0 + 32 * (warp & 3), n < p.a.n && m < p.a.M ? v : 0.0f);
+    }
+  };
+  if (warp >= 4) {
+    if (p.a.bias && n < p.a.n) {
+      b0 = p.a.bias[n];
+      if (GLU) b1 = p.a.bias[p.a.n + n];
+    }
+    have = mbar_wait(acc_full, 0, p.a.err, T0B_DEVERR_WAIT_ACC, abort_flag) && !*abort_flag;
+    have = __all_sync(0xFFFFFFFFu, have);
+    tc_fence_after();
+    for (int t0 = 0; t0 < toks && have; t0 += 8) {
+      float g[8], u[8];
+      tmem_ld8(trow + t0, g);
+      if (GLU) tmem_ld8(trow + NT + t0, u);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int t = t0 + j;
+        if (t >= toks) break;
+        if (CS == 1) {
+          finish(t, g[j], GLU ? u[j] : 0.0f);
+        } else {
+          const int owner = t / share;
+          const uint32_t at = mapa_shared(smem_u32(smem + p.off_slot) + ((rank * share + t - owner * share) * H * 128 + row) * 4, owner);
+          st_cluster_f32(at, g[j]);
+          if (GLU) st_cluster_f32(at + 512, u[j]);
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncwarp();
+  if (CS > 1) {
+    cluster_sync_all();
+    if (warp >= 4 && have) {
+      const float *slot = reinterpret_cast<const float *>(smem + p.off_slot) + row;
+      for (int t = rank * share; t < min(toks, (rank + 1) * share); ++t) {
+        float g = 0.0f, u = 0.0f;
+        for (int c = 0; c < CS; ++c) {
+          const float *v = slot + (c * share + t - rank * share) * H * 128;
+          g += v[0];
+          if (GLU) u += v[128];
+        }
+        finish(t, g, u);
+      }
+    }
+  } else {
+    __syncthreads();
+  }
+  if (GLU && p.out_type < 0 && warp >= 4 && m0 + NT >= p.a.M)  // zero scales of the row group's rows behind the last token
+    for (int m = p.a.M + rank; m < (p.a.M + 127) / 128 * 128; m += CS) quantize_lanes<NV>(p.a.q, m, n0 + 32 * (warp & 3), 0.0f);
+  __syncwarp();
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(p.tmem_cols) : "memory");
+  }
+}
+
 // ------------------------------------------------------------- host side
 // Every kernel here starts while the previous one of the stream ends and
 // waits for it (griddepcontrol.wait) before its first access to memory that a
@@ -712,11 +1088,11 @@ cudaError_t launch(void (*k)(P...), dim3 grid, dim3 block, cudaStream_t st, A...
   return cudaLaunchKernelEx(&cfg, k, args...);
 }
 
-// Tensor maps of a matrix: codes in boxes of 128 rows x 128 bytes, scales in
+// Tensor maps of a matrix: codes in boxes of `rows` rows x 128 bytes, scales in
 // boxes of one row group's `at` tiles.
-bool code_map(CUtensorMap *tm, const Fp4Mat &q) {
+bool code_map(CUtensorMap *tm, const Fp4Mat &q, int rows) {
   const uint64_t pitch = (uint64_t)((q.k + 31) / 32) * 16;
-  return t0b_make_tmap_u8_2d(tm, q.codes, pitch, (uint64_t)q.rows, pitch, 128, 128);
+  return t0b_make_tmap_u8_2d(tm, q.codes, pitch, (uint64_t)q.rows, pitch, 128, rows);
 }
 bool scale_map(CUtensorMap *tm, const Fp4Mat &q, int kt, int at) {
   return t0b_make_tmap_f16_3d(tm, q.scales, 256, (uint64_t)kt, (uint64_t)((q.rows + 127) / 128), 512, (uint64_t)kt * 512, 256,
@@ -744,6 +1120,92 @@ int max_pairs(const void *kfn, const cudaLaunchConfig_t &cfg) {
   return n;
 }
 
+bool rows_aligned(const void *p, int64_t ld, int type) { return ((uintptr_t)p | (uint64_t)ld * (type == TY_F32 ? 4 : 2)) % 16 == 0; }
+
+// How a product is divided for the split kernel.
+struct SplitPlan {
+  int NT, CS, SL, rt;
+  int64_t ctas;
+};
+int sm_count() {
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+  return n;
+}
+SplitPlan split_plan(bool glu, int M, int n, int K, int sms) {
+  SplitPlan q;
+  const int most = glu ? 64 : 128;  // tokens of a tile; several tiles start at whole scale columns
+  q.NT = M <= most ? (M + 7) / 8 * 8 : most;
+  q.rt = (n + 127) / 128;
+  const int64_t tiles = (int64_t)q.rt * ((M + q.NT - 1) / q.NT);
+  const int S = (K + 255) / 256;
+  int cs = 1;
+  while (cs < SPLIT_MAX_CLUSTER && tiles * cs * 2 <= sms && S >= cs * 2) cs *= 2;
+  q.SL = (S + cs - 1) / cs;
+  q.CS = (S + q.SL - 1) / q.SL;
+  q.ctas = tiles * q.CS;
+  return q;
+}
+
+// x_type < 0: x is the 4-bit matrix xm; else plain, to be quantised as xm says.
+template <bool NV, bool GLU, bool FUSED>
+cudaError_t launch_split(const Fp4Mat &w, const Fp4Mat &xm, const void *x, int x_type, int64_t ldx, const Fp4Args &a, int out_type,
+                         const SplitPlan &q, bool early, cudaStream_t st) {
+  constexpr int AT = NV ? 4 : 2, H = GLU ? 2 : 1;
+  constexpr uint32_t SC = AT * 512, LIMIT = 232448;
+  SplitArgs p{};
+  p.a = a;
+  p.NT = q.NT, p.CS = q.CS, p.SL = q.SL, p.rt = q.rt;
+  p.out_type = out_type;
+  p.rot = GLU && a.up_row % 128;
+  p.early = early;
+  p.x = x, p.x_type = x_type, p.ldx = ldx, p.x_ts = xm.ts;
+  p.xvec = FUSED && rows_aligned(x, ldx, x_type);
+  p.stage = split_stage<NV, GLU, FUSED>(q.NT);
+  const uint32_t fixed = (FUSED ? (uint32_t)q.SL * (q.NT * 128 + SC) : 0) +
+                         (q.CS > 1 ? (uint32_t)((q.NT + q.CS - 1) / q.CS * q.CS) * H * 512 : 0) + 512 + 1024;
+  // Tensor memory is given out CTA by CTA: clusters that hold some on one SM
+  // and wait for more on another could wait for each other.  So no two CTAs
+  // whose columns exceed the 512 fit on an SM: up to 256 columns with over a
+  // third of its shared memory, more with over two thirds.
+  auto columns = [&] { return H * q.NT + p.NS * AT * 4 * (H + 1); };
+  p.NS = q.SL < SPLIT_MAX_NS ? q.SL : SPLIT_MAX_NS;
+  while (p.NS > 4 && columns() > 256) --p.NS;
+  while (p.NS > 1 && p.NS * p.stage + fixed > LIMIT) --p.NS;
+  const uint32_t used = p.NS * p.stage + fixed, least = columns() <= 256 ? 76 * 1024 : 152 * 1024;
+  const uint32_t smem = used > least ? used : least;
+  if (smem > LIMIT) return cudaErrorInvalidConfiguration;
+  p.off_x = p.NS * p.stage;
+  p.off_xs = p.off_x + (FUSED ? q.SL * q.NT * 128 : 0);
+  p.off_slot = p.off_xs + (FUSED ? q.SL * SC : 0);
+  p.off_bar = used - 512 - 1024;
+  for (p.tmem_cols = 32; (int)p.tmem_cols < columns();) p.tmem_cols *= 2;
+  if (p.tmem_cols > 512 || q.ctas > INT32_MAX) return cudaErrorInvalidConfiguration;
+  CUtensorMap tx, tw, txs, tws;
+  if (!code_map(&tw, w, 128) || !scale_map(&tws, w, a.kt, AT)) return cudaErrorInvalidValue;
+  if (FUSED)
+    tx = tw, txs = tws;  // not used
+  else if (!code_map(&tx, xm, q.NT) || !scale_map(&txs, xm, a.kt, AT))
+    return cudaErrorInvalidValue;
+  auto kfn = fp4_gemm_split_kernel<NV, GLU, FUSED>;
+  cudaError_t e = t0b_smem_limit((const void *)kfn, smem);
+  if (e != cudaSuccess) return e;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = q.CS;
+  at[0].val.clusterDim.y = 1;
+  at[0].val.clusterDim.z = 1;
+  at[1] = dependent_launch();
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)q.ctas);
+  cfg.blockDim = dim3(SPLIT_THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = at;
+  cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, kfn, tx, tw, txs, tws, p);
+}
+
 template <bool NV, bool GLU, bool ROT, int TY>
 cudaError_t launch_pair(const Fp4Mat &w, const Fp4Mat &x, Fp4Args p, cudaStream_t st) {
   using C = PairCfg<NV, ROT>;
@@ -756,7 +1218,7 @@ cudaError_t launch_pair(const Fp4Mat &w, const Fp4Mat &x, Fp4Args p, cudaStream_
   cudaError_t e = t0b_smem_limit((const void *)kfn, C::SMEM);
   if (e != cudaSuccess) return e;
   CUtensorMap tx, tw, txs, tws;
-  if (!code_map(&tx, x) || !code_map(&tw, w) || !scale_map(&txs, x, p.kt, C::AT) || !scale_map(&tws, w, p.kt, C::AT))
+  if (!code_map(&tx, x, 128) || !code_map(&tw, w, 128) || !scale_map(&txs, x, p.kt, C::AT) || !scale_map(&tws, w, p.kt, C::AT))
     return cudaErrorInvalidValue;
   CUtensorMap ty = tx;  // not used without aligned rows
   if (p.vec && !t0b_make_tmap_rows64(&ty, p.y, TY == TY_F32 ? 4 : 2, (uint64_t)p.n, (uint64_t)p.M, (uint64_t)p.ld))
@@ -798,8 +1260,6 @@ cudaError_t gemm_fmt(const Fp4Mat &w, const Fp4Mat &x, const Fp4Out &out, const 
   return gemm_ty<NV, TY_BF16>(w, x, out, p, st);
 }
 
-bool rows_aligned(const void *p, int64_t ld, int type) { return ((uintptr_t)p | (uint64_t)ld * (type == TY_F32 ? 4 : 2)) % 16 == 0; }
-
 // Rows of one scale tile's width get the lanes of one tile, longer ones a warp.
 template <int TY, bool NV, bool QUANT>
 cudaError_t convert(const void *x, int64_t ld, const Fp4Mat &q, cudaStream_t st) {
@@ -833,7 +1293,9 @@ cudaError_t t0b_launch_fp4_dequantize(const Fp4Mat &q, int y_type, void *y, int6
   return q.blk == 16 ? convert_ty<true, false>(y_type, y, ldy, q, st) : convert_ty<false, false>(y_type, y, ldy, q, st);
 }
 
-cudaError_t t0b_launch_fp4_gemm(const Fp4Mat &w, const Fp4Mat &x, const Fp4Out &out, int *err, cudaStream_t st) {
+namespace {
+
+Fp4Args product_args(const Fp4Mat &w, const Fp4Mat &x, const Fp4Out &out, int *err) {
   Fp4Args p{};
   p.M = x.rows;
   p.n = out.glu ? w.rows / 2 : w.rows;
@@ -847,5 +1309,48 @@ cudaError_t t0b_launch_fp4_gemm(const Fp4Mat &w, const Fp4Mat &x, const Fp4Out &
   p.up_row = out.glu ? p.n : 0;
   p.err = err;
   p.vec = !out.quant && rows_aligned(out.y, out.ld, out.type);
-  return w.blk == 16 ? gemm_fmt<true>(w, x, out, p, st) : gemm_fmt<false>(w, x, out, p, st);
+  return p;
+}
+
+// Tokens up to which a CTA of the split kernel quantises plain activations
+// itself.
+constexpr int FUSED_MAX_TOKENS = 32;
+
+bool use_split(const Fp4Args &a, bool glu, const SplitPlan &q, int sms) {
+  const int64_t pair_tiles = (int64_t)((a.M + 255) / 256) * (glu ? (a.n + 127) / 128 : (a.n + 255) / 256);
+  (void)q;
+  return a.M <= 256 || 4 * pair_tiles <= sms;
+}
+
+template <bool FUSED>
+cudaError_t split_dispatch(const Fp4Mat &w, const Fp4Mat &xm, const void *x, int x_type, int64_t ldx, const Fp4Out &out,
+                           const Fp4Args &a, const SplitPlan &q, bool early, cudaStream_t st) {
+  const int ot = out.quant ? -1 : out.type;
+  if (w.blk == 16)
+    return out.glu ? launch_split<true, true, FUSED>(w, xm, x, x_type, ldx, a, ot, q, early, st)
+                   : launch_split<true, false, FUSED>(w, xm, x, x_type, ldx, a, ot, q, early, st);
+  return out.glu ? launch_split<false, true, FUSED>(w, xm, x, x_type, ldx, a, ot, q, early, st)
+                 : launch_split<false, false, FUSED>(w, xm, x, x_type, ldx, a, ot, q, early, st);
+}
+
+}  // namespace
+
+cudaError_t t0b_launch_fp4_gemm(const Fp4Mat &w, const Fp4Mat &x, const Fp4Out &out, bool after_own, int *err, cudaStream_t st) {
+  const Fp4Args a = product_args(w, x, out, err);
+  const int sms = sm_count();
+  const SplitPlan q = split_plan(out.glu, a.M, a.n, a.K, sms);
+  if (use_split(a, out.glu, q, sms)) return split_dispatch<false>(w, x, nullptr, -1, 0, out, a, q, after_own, st);
+  return w.blk == 16 ? gemm_fmt<true>(w, x, out, a, st) : gemm_fmt<false>(w, x, out, a, st);
+}
+
+cudaError_t t0b_launch_fp4_linear(const Fp4Mat &w, int x_type, const void *x, int64_t ldx, const Fp4Mat &xq, const Fp4Out &out,
+                                  int *err, cudaStream_t st) {
+  if (xq.rows <= FUSED_MAX_TOKENS) {
+    const Fp4Args a = product_args(w, xq, out, err);
+    const SplitPlan q = split_plan(out.glu, a.M, a.n, a.K, sm_count());
+    // its share of the activations stays in shared memory
+    if (q.SL <= 8) return split_dispatch<true>(w, xq, x, x_type, ldx, out, a, q, false, st);
+  }
+  const cudaError_t e = t0b_launch_fp4_quantize(x_type, x, ldx, xq, st);
+  return e != cudaSuccess ? e : t0b_launch_fp4_gemm(w, xq, out, true, err, st);
 }

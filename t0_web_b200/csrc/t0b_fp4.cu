@@ -157,7 +157,7 @@ extern "C" t0b_status t0b_fp4_gemm(t0b_engine *e, const t0b_fp4 *w, const t0b_fp
   DeviceScope dev(t0b_engine_device(e));
   TRY(cuda_status(fn, dev.status));
   const Fp4Out out{y_type, y_dev, ldy, bias_dev, false, false, {}};
-  return cuda_status(fn, t0b_launch_fp4_gemm(wm, xm, out, t0b_engine_fp4_err(e), (cudaStream_t)stream));
+  return cuda_status(fn, t0b_launch_fp4_gemm(wm, xm, out, false, t0b_engine_fp4_err(e), (cudaStream_t)stream));
 }
 
 extern "C" t0b_status t0b_fp4_glu(t0b_engine *e, const t0b_fp4 *w, const t0b_fp4 *x, const float *bias_dev, int z_type,
@@ -182,7 +182,7 @@ extern "C" t0b_status t0b_fp4_glu(t0b_engine *e, const t0b_fp4 *w, const t0b_fp4
   }
   DeviceScope dev(t0b_engine_device(e));
   TRY(cuda_status(fn, dev.status));
-  return cuda_status(fn, t0b_launch_fp4_gemm(wm, xm, out, t0b_engine_fp4_err(e), (cudaStream_t)stream));
+  return cuda_status(fn, t0b_launch_fp4_gemm(wm, xm, out, false, t0b_engine_fp4_err(e), (cudaStream_t)stream));
 }
 
 extern "C" t0b_status t0b_fp4_linear(t0b_engine *e, const t0b_fp4 *w, int x_type, const void *x_dev, int64_t ldx,
@@ -199,10 +199,8 @@ extern "C" t0b_status t0b_fp4_linear(t0b_engine *e, const t0b_fp4 *w, int x_type
   TRY(check_plain(fn, "y", y_type, y_dev, ldy, xm.rows, wm.rows));
   DeviceScope dev(t0b_engine_device(e));
   TRY(cuda_status(fn, dev.status));
-  const cudaStream_t st = (cudaStream_t)stream;
-  TRY(cuda_status(fn, t0b_launch_fp4_quantize(x_type, x_dev, ldx, xm, st)));
   const Fp4Out out{y_type, y_dev, ldy, bias_dev, false, false, {}};
-  return cuda_status(fn, t0b_launch_fp4_gemm(wm, xm, out, t0b_engine_fp4_err(e), st));
+  return cuda_status(fn, t0b_launch_fp4_linear(wm, x_type, x_dev, ldx, xm, out, t0b_engine_fp4_err(e), (cudaStream_t)stream));
 }
 
 extern "C" t0b_status t0b_fp4_mlp(t0b_engine *e, const t0b_fp4 *w0, const t0b_fp4 *w2, int x_type, const void *x_dev,
@@ -228,11 +226,10 @@ extern "C" t0b_status t0b_fp4_mlp(t0b_engine *e, const t0b_fp4 *w0, const t0b_fp
   TRY(cuda_status(fn, dev.status));
   const cudaStream_t st = (cudaStream_t)stream;
   int *err = t0b_engine_fp4_err(e);
-  TRY(cuda_status(fn, t0b_launch_fp4_quantize(x_type, x_dev, ldx, xm, st)));
   const Fp4Out hid{0, nullptr, 0, b0_dev, true, true, zm};
-  TRY(cuda_status(fn, t0b_launch_fp4_gemm(w0m, xm, hid, err, st)));
+  TRY(cuda_status(fn, t0b_launch_fp4_linear(w0m, x_type, x_dev, ldx, xm, hid, err, st)));
   const Fp4Out out{y_type, y_dev, ldy, b2_dev, false, false, {}};
-  return cuda_status(fn, t0b_launch_fp4_gemm(w2m, zm, out, err, st));
+  return cuda_status(fn, t0b_launch_fp4_gemm(w2m, zm, out, true, err, st));
 }
 
 extern "C" t0b_status t0b_fp4_sync(t0b_engine *e, void *stream) {

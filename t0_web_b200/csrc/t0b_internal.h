@@ -146,4 +146,11 @@ struct Fp4Out {
 };
 cudaError_t t0b_launch_fp4_quantize(int x_type, const void *x, int64_t ldx, const Fp4Mat &out, cudaStream_t st);
 cudaError_t t0b_launch_fp4_dequantize(const Fp4Mat &in, int y_type, void *y, int64_t ldy, cudaStream_t st);
-cudaError_t t0b_launch_fp4_gemm(const Fp4Mat &w, const Fp4Mat &x, const Fp4Out &out, int *err, cudaStream_t st);
+// after_own: the kernel queued before it on `st` is one of these launchers'
+// and writes none of w (whose tiles may then be fetched while it still runs).
+cudaError_t t0b_launch_fp4_gemm(const Fp4Mat &w, const Fp4Mat &x, const Fp4Out &out, bool after_own, int *err,
+                                cudaStream_t st);
+// The product on plain activations, quantised as xq says (its memory is used
+// where the product reads 4-bit activations from memory).
+cudaError_t t0b_launch_fp4_linear(const Fp4Mat &w, int x_type, const void *x, int64_t ldx, const Fp4Mat &xq,
+                                  const Fp4Out &out, int *err, cudaStream_t st);

@@ -367,18 +367,18 @@ def test_graph_replay_and_streams(engine, m):
         torch.cuda.synchronize()
         with torch.cuda.graph(g, stream=s):
             fp4.mlp(engine, w0, w2, x, xq, zq, y)
-        graphs.append((g, s, x, y))
+        graphs.append((g, s, x, y, xq, zq))  # a graph's buffers live as long as it does
     torch.cuda.synchronize()
     other, (oxq, ozq, oy) = torch.cuda.Stream(), bufs()
     for i in range(4):
-        for j, (g, s, x, y) in enumerate(graphs):
+        for j, (g, s, x, y, *_) in enumerate(graphs):
             with torch.cuda.stream(s):
                 x.copy_(xs[(i + j) % 4])
                 g.replay()
         with torch.cuda.stream(other):
             fp4.mlp(engine, w0, w2, xs[3 - i], oxq, ozq, oy)
         torch.cuda.synchronize()
-        for j, (g, s, x, y) in enumerate(graphs):
+        for j, (g, s, x, y, *_) in enumerate(graphs):
             assert torch.equal(y, want[(i + j) % 4])
         assert torch.equal(oy, want[3 - i])
     fp4.sync(engine)
