@@ -784,9 +784,11 @@ T0B_DEV void umma_fp4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32
 T0B_DEV void umma_commit(uint64_t *bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
-T0B_DEV void st_cluster_f32(uint32_t addr, float v) {
-  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
+T0B_DEV void st_cluster_f32x4(uint32_t addr, const float *v) {
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3])
+               : "memory");
 }
+T0B_DEV void add4(float4 &a, const float4 &b) { a.x += b.x, a.y += b.y, a.z += b.z, a.w += b.w; }
 
 // Bytes of a stage: weight codes, weight scales (gated: two halves, and room
 // for the up rows' scales as they are held), then, unless FUSED, the tokens'.
@@ -994,45 +996,47 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 1)
   if (CS > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
 
   // ------------------------------------------------------------ results
-  const int row = 32 * (warp & 3) + lane, n = n0 + row;  // warps 4 .. 7: this thread's weight row
-  const int share = (NT + CS - 1) / CS;                  // tokens whose slices this CTA adds
+  // Warps 0 .. 3 and 4 .. 7 take alternate groups of eight tokens; a thread has
+  // one weight row.  The slices' partial sums go to the CTA that adds them as
+  // [source][four tokens][gate, up][row][token], 16 bytes a thread.
+  const int half = warp >> 2, row = 32 * (warp & 3) + lane, n = n0 + row;
+  const int sh4 = ((NT + CS - 1) / CS + 3) / 4;  // groups of four tokens whose slices a CTA adds
   const uint32_t trow = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
-  bool have = true;
   float b0 = 0.0f, b1 = 0.0f;
+  if (p.a.bias && n < p.a.n) {
+    b0 = p.a.bias[n];
+    if (GLU) b1 = p.a.bias[p.a.n + n];
+  }
   auto finish = [&](int t, float g, float u) {  // token t of the tile
     const int m = m0 + t;
     float v = fmaf(g, p.a.alpha, b0);
     if constexpr (GLU) v = silu_mul(v, fmaf(u, p.a.alpha, b1));
     if (p.out_type >= 0) {
-      if (n < p.a.n && m < p.a.M) store_elem(p.a.y, p.out_type, m * p.a.ld + n, v);
+      if (n < p.a.n) store_elem(p.a.y, p.out_type, m * p.a.ld + n, v);
     } else if constexpr (GLU) {
-      quantize_lanes<NV>(p.a.q, m, n0 + 32 * (warp & 3), n < p.a.n && m < p.a.M ? v : 0.0f);
+      quantize_lanes<NV>(p.a.q, m, n0 + 32 * (warp & 3), n < p.a.n ? v : 0.0f);
     }
   };
-  if (warp >= 4) {
-    if (p.a.bias && n < p.a.n) {
-      b0 = p.a.bias[n];
-      if (GLU) b1 = p.a.bias[p.a.n + n];
-    }
-    have = mbar_wait(acc_full, 0, p.a.err, T0B_DEVERR_WAIT_ACC, abort_flag) && !*abort_flag;
-    have = __all_sync(0xFFFFFFFFu, have);
-    tc_fence_after();
-    for (int t0 = 0; t0 < toks && have; t0 += 8) {
-      float g[8], u[8];
-      tmem_ld8(trow + t0, g);
-      if (GLU) tmem_ld8(trow + NT + t0, u);
+  bool have = mbar_wait(acc_full, 0, p.a.err, T0B_DEVERR_WAIT_ACC, abort_flag) && !*abort_flag;
+  have = __all_sync(0xFFFFFFFFu, have);
+  tc_fence_after();
+  for (int t0 = 8 * half; t0 < toks && have; t0 += 16) {
+    float g[8], u[8];
+    tmem_ld8(trow + t0, g);
+    if (GLU) tmem_ld8(trow + NT + t0, u);
+    if (CS == 1) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int t = t0 + j;
-        if (t >= toks) break;
-        if (CS == 1) {
-          finish(t, g[j], GLU ? u[j] : 0.0f);
-        } else {
-          const int owner = t / share;
-          const uint32_t at = mapa_shared(smem_u32(smem + p.off_slot) + ((rank * share + t - owner * share) * H * 128 + row) * 4, owner);
-          st_cluster_f32(at, g[j]);
-          if (GLU) st_cluster_f32(at + 512, u[j]);
-        }
+      for (int j = 0; j < 8; ++j)
+        if (t0 + j < toks) finish(t0 + j, g[j], GLU ? u[j] : 0.0f);
+    } else {
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int c4 = t0 / 4 + c, owner = c4 / sh4;
+        if (owner >= CS) break;
+        const uint32_t at =
+            mapa_shared(smem_u32(smem + p.off_slot) + (((rank * sh4 + c4 - owner * sh4) * H) * 128 + row) * 16, owner);
+        st_cluster_f32x4(at, g + 4 * c);
+        if (GLU) st_cluster_f32x4(at + 2048, u + 4 * c);
       }
     }
   }
@@ -1040,23 +1044,34 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 1)
   __syncwarp();
   if (CS > 1) {
     cluster_sync_all();
-    if (warp >= 4 && have) {
-      const float *slot = reinterpret_cast<const float *>(smem + p.off_slot) + row;
-      for (int t = rank * share; t < min(toks, (rank + 1) * share); ++t) {
-        float g = 0.0f, u = 0.0f;
-        for (int c = 0; c < CS; ++c) {
-          const float *v = slot + (c * share + t - rank * share) * H * 128;
-          g += v[0];
-          if (GLU) u += v[128];
-        }
-        finish(t, g, u);
+    const float4 *slot = reinterpret_cast<const float4 *>(smem + p.off_slot) + row;
+    for (int c4 = half; c4 < sh4 && have; c4 += 2) {
+      const int t0 = 4 * (rank * sh4 + c4);
+      if (t0 >= toks) break;
+      float4 g = make_float4(0.f, 0.f, 0.f, 0.f), u = g;
+#pragma unroll
+      for (int c = 0; c < SPLIT_MAX_CLUSTER; ++c) {
+        if (c >= CS) break;
+        const float4 *v = slot + (c * sh4 + c4) * H * 128;
+        add4(g, v[0]);
+        if (GLU) add4(u, v[128]);
       }
+      finish(t0, g.x, u.x);
+      if (t0 + 1 < toks) finish(t0 + 1, g.y, u.y);
+      if (t0 + 2 < toks) finish(t0 + 2, g.z, u.z);
+      if (t0 + 3 < toks) finish(t0 + 3, g.w, u.w);
     }
   } else {
     __syncthreads();
   }
-  if (GLU && p.out_type < 0 && warp >= 4 && m0 + NT >= p.a.M)  // zero scales of the row group's rows behind the last token
-    for (int m = p.a.M + rank; m < (p.a.M + 127) / 128 * 128; m += CS) quantize_lanes<NV>(p.a.q, m, n0 + 32 * (warp & 3), 0.0f);
+  if (GLU && p.out_type < 0 && m0 + NT >= p.a.M && rank == 0) {
+    // zero scales of the last row group's rows behind the last token
+    const int m = p.a.M + (int)threadIdx.x % 128;
+    constexpr int TILES = NV ? 2 : 1;  // scale tiles of 128 columns
+    const int t = n0 / 128 * TILES + (int)threadIdx.x / 128, kt = (p.a.q.k + (NV ? 63 : 127)) / (NV ? 64 : 128);
+    if (m < (p.a.M + 127) / 128 * 128 && (int)threadIdx.x / 128 < TILES && t < kt)
+      *reinterpret_cast<uint32_t *>(p.a.q.scales + scale_at(m, 4 * t, kt)) = 0;
+  }
   __syncwarp();
   if (warp == 1) {
     tc_fence_after();
@@ -1163,7 +1178,7 @@ cudaError_t launch_split(const Fp4Mat &w, const Fp4Mat &xm, const void *x, int x
   p.xvec = FUSED && rows_aligned(x, ldx, x_type);
   p.stage = split_stage<NV, GLU, FUSED>(q.NT);
   const uint32_t fixed = (FUSED ? (uint32_t)q.SL * (q.NT * 128 + SC) : 0) +
-                         (q.CS > 1 ? (uint32_t)((q.NT + q.CS - 1) / q.CS * q.CS) * H * 512 : 0) + 512 + 1024;
+                         (q.CS > 1 ? (uint32_t)(((q.NT + q.CS - 1) / q.CS + 3) / 4 * q.CS) * H * 2048 : 0) + 512 + 1024;
   // Tensor memory is given out CTA by CTA: clusters that hold some on one SM
   // and wait for more on another could wait for each other.  So no two CTAs
   // whose columns exceed the 512 fit on an SM: up to 256 columns with over a
