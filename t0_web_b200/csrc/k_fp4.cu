@@ -81,61 +81,61 @@ T0B_DEV void values8(uint32_t w, float *v) {
   }
 }
 
-// max(a, |b|) that keeps a NaN (as bits above infinity's).
-T0B_DEV float absmax(float a, float b) {
+// The largest of a and two magnitudes; keeps a NaN (as bits above infinity's).
+T0B_DEV float absmax(float a, float b, float c) {
   float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(fabsf(b)));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(fabsf(b)), "f"(fabsf(c)));
   return r;
 }
-// A block's scale byte and the factors that divide by its scale, from the bits
-// of its largest magnitude (infinities and NaNs compare above every finite
-// value).  The quotients are correctly rounded, so that every rounding to 4
-// bits is decided as if it were exact: with power-of-two scales the product
-// with 1 / d is exact; otherwise d has four significant bits, a quotient that
-// is not itself a border differs from it by more than half an ulp, and one
-// residual step (x - u d is exact in an FMA, 1 / d correctly rounded) gives
-// the correctly rounded quotient.
+template <int N>
+T0B_DEV float absmax_of(const float *v) {
+  float t = 0.0f;
+#pragma unroll
+  for (int i = 0; i < N; i += 2) t = absmax(t, v[i], v[i + 1]);
+  return t;
+}
+// A block's scale byte and the division by its scale, from the bits of its
+// largest magnitude (infinities and NaNs compare above every finite value).
+// Every rounding to 4 bits is decided as by the exact quotient.  MX: the
+// product with 1 / d is exact.  NV: d has four significant bits; 1 / d is held
+// as hi + lo to 2^-44, so u = fma(x, hi, x lo) is the quotient rounded to f32
+// (a quotient on a border is representable and comes out as itself, one that
+// is not differs from the border by at least 1.06 half ulps).  lo >= 0: the
+// sign of a zero and of an overflow stays.
 template <bool NV>
 struct BlockScale {
   uint32_t byte;
-  float d, rcp;
-  bool clamp;  // quotients that may overflow (only where the scale is at its largest)
-  T0B_DEV BlockScale(uint32_t amax, float ts) {
-    clamp = false;
+  float hi, lo;
+  T0B_DEV BlockScale(uint32_t amax, const Fp4Mat &q) {
     if constexpr (!NV) {
       byte = amax >= 0x7F800000u ? 255u : max(amax >> 23, 2u) - 2u;
-      rcp = __uint_as_float((254u - min(byte, 252u)) << 23);
-      d = 0.0f;
+      hi = __uint_as_float((254u - min(byte, 252u)) << 23);
+      lo = 0.0f;
     } else {
       const float a = __uint_as_float(amax);
-      byte = amax >= 0x7F800000u ? 127u : e4m3_of(__fdiv_rn(a, 6.0f * ts));
-      d = e4m3_value(byte) * ts;
-      rcp = byte ? __frcp_rn(d) : 0.0f;  // a scale of zero: all values zero
-      clamp = a > 16.0f * d && byte;
+      byte = e4m3_of(fmaf(a, q.r6_hi, a * q.r6_lo));  // a / (6 tensor_scale), the same way
+      if (amax >= 0x7F800000u) byte = 127u;
+      const float d = e4m3_value(byte) * q.ts;
+      float r;
+      asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
+      hi = byte ? __uint_as_float(__float_as_uint(r) - 4u) : 0.0f;  // below 1 / d
+      lo = fmaf(-hi, d, 1.0f) * hi;
     }
   }
   T0B_DEV float quotient(float x) const {
-    if constexpr (!NV) return x * rcp;
-    const float u = x * rcp;
-    return fmaf(-fmaf(u, d, -x), rcp, u);  // this order keeps the sign of a zero
+    if constexpr (!NV) return x * hi;
+    return fmaf(x, hi, x * lo);
   }
 };
 
 // Eight values of a block to a word of codes.
 template <bool NV>
-T0B_DEV void quantize8(const BlockScale<NV> &s, const float *v, uint32_t *w) {
+T0B_DEV uint32_t quantize8(const BlockScale<NV> &s, const float *v) {
   float u[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) u[j] = s.quotient(v[j]);
-  if constexpr (NV) {
-    if (s.clamp)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) u[j] = s.quotient(fminf(fmaxf(v[j], -8.0f * s.d), 8.0f * s.d));
-    if (s.byte == 0)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) u[j] = 0.0f;  // no signs either
-  }
-  *w = codes8(u);
+  const uint32_t w = codes8(u);
+  return NV && s.byte == 0 ? 0u : w;  // a scale of zero: no signs either
 }
 
 // ------------------------------------------------------------ quantisation
@@ -185,27 +185,24 @@ __global__ void __launch_bounds__(32 * QT_WARPS) fp4_quantize_kernel(const typen
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[i][j] = 0.0f;
   }
-  uint32_t sc[4];
+  uint32_t sc = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    float top = 0.0f;
+    float top = absmax_of<8>(v[i]);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) top = absmax(top, v[i][j]);
-    uint32_t amax = __float_as_uint(top);
-#pragma unroll
-    for (int o = 1; o < LB; o *= 2) amax = max(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, o));
-    const BlockScale<NV> s(amax, q.ts);
-    sc[i] = s.byte << (8 * (lane / LB % 4));
-    sc[i] |= __shfl_xor_sync(0xFFFFFFFFu, sc[i], LB);
-    sc[i] |= __shfl_xor_sync(0xFFFFFFFFu, sc[i], 2 * LB);
-    uint32_t w;
-    quantize8<NV>(s, v[i], &w);
+    for (int o = 1; o < LB; o *= 2) top = absmax(top, __shfl_xor_sync(0xFFFFFFFFu, top, o), 0.0f);
+    const BlockScale<NV> s(__float_as_uint(top), q);
+    sc |= s.byte << (8 * i);
     if (r + 32 * i < q.rows && k0 / 2 < (int)code_pitch(q.k))
-      *reinterpret_cast<uint32_t *>(q.codes + (r + 32 * i) * code_pitch(q.k) + k0 / 2) = w;
+      *reinterpret_cast<uint32_t *>(q.codes + (r + 32 * i) * code_pitch(q.k) + k0 / 2) = quantize8<NV>(s, v[i]);
   }
+  // sc: one block of four rows; the tile's words are four blocks of one row
+  const int b = lane / LB % 4;
+  sc = __byte_perm(sc, __shfl_xor_sync(0xFFFFFFFFu, sc, LB), b & 1 ? 0x3715 : 0x6240);
+  sc = __byte_perm(sc, __shfl_xor_sync(0xFFFFFFFFu, sc, 2 * LB), b & 2 ? 0x3276 : 0x5410);
   const int t = k0 / (4 * BLK);
-  if (lane % (4 * LB) == 0 && t < kt && group < (q.rows + 127) / 128)
-    *reinterpret_cast<uint4 *>(q.scales + ((size_t)group * kt + t) * 512 + (r & 31) * 16) = make_uint4(sc[0], sc[1], sc[2], sc[3]);
+  if (lane % LB == 0 && t < kt && group < (q.rows + 127) / 128)
+    *reinterpret_cast<uint32_t *>(q.scales + ((size_t)group * kt + t) * 512 + (r & 31) * 16 + 4 * b) = sc;
 }
 
 // ----------------------------------------------------------- the other way
@@ -408,14 +405,10 @@ T0B_DEV void store_quant32(const Fp4Mat &q, int r, int c0, float *v) {
   uint32_t w[4], sc = 0;
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
-    float top = 0.0f;
-#pragma unroll
-    for (int j = 0; j < BLK; ++j) top = absmax(top, v[b * BLK + j]);
-    const uint32_t amax = __float_as_uint(top);
-    const BlockScale<NV> s(amax, q.ts);
+    const BlockScale<NV> s(__float_as_uint(absmax_of<BLK>(v + b * BLK)), q);
     sc |= s.byte << (8 * b);
 #pragma unroll
-    for (int i = 0; i < BLK / 8; ++i) quantize8<NV>(s, v + b * BLK + 8 * i, w + b * BLK / 8 + i);
+    for (int i = 0; i < BLK / 8; ++i) w[b * BLK / 8 + i] = quantize8<NV>(s, v + b * BLK + 8 * i);
   }
   uint8_t *ps = q.scales + scale_at(r, c0 / BLK, kt);
   if (NV)
@@ -717,7 +710,7 @@ struct SplitArgs {
   const void *x;            // FUSED
   int x_type;
   int64_t ldx;
-  float x_ts;
+  Fp4Mat xq;                // its scales' constants
   int xvec;
 };
 
@@ -737,16 +730,15 @@ template <bool NV>
 T0B_DEV void quantize_lanes(const Fp4Mat &q, int r, int c0, float v) {
   constexpr int BLK = NV ? 16 : 32;
   const int lane = threadIdx.x & 31, kt = (q.k + 4 * BLK - 1) / (4 * BLK);
-  float top = absmax(0.0f, v);
+  float top = fabsf(v);
 #pragma unroll
-  for (int o = BLK / 2; o; o >>= 1) top = absmax(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-  const BlockScale<NV> s(__float_as_uint(top), q.ts);
+  for (int o = BLK / 2; o; o >>= 1) top = absmax(top, __shfl_xor_sync(0xFFFFFFFFu, top, o), 0.0f);
+  const BlockScale<NV> s(__float_as_uint(top), q);
   // eight lanes' values to every eighth lane
   float u[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) u[j] = __shfl_sync(0xFFFFFFFFu, v, (lane & 24) + j);
-  uint32_t w;
-  quantize8<NV>(s, u, &w);
+  const uint32_t w = quantize8<NV>(s, u);
   const int b = (c0 + lane) / BLK;
   if (lane % BLK == 0 && b < 4 * kt) q.scales[scale_at(r, b, kt)] = r < q.rows && b * BLK < q.k ? (uint8_t)s.byte : 0;
   if (lane % 8 == 0 && r < q.rows && (c0 + lane) / 2 < (int)code_pitch(q.k))
@@ -818,14 +810,11 @@ T0B_DEV void quantize_slice(const SplitArgs &p, uint8_t *codes, uint8_t *scales,
       const int i = i0 + u * (SPLIT_THREADS / 32);
       if (i >= n) break;
       const int t = i / stages, s = i % stages;
-      float top = 0.0f;
+      float top = absmax_of<8>(v[u]);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) top = absmax(top, v[u][j]);
-#pragma unroll
-      for (int o = 1; o < LB; o *= 2) top = absmax(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-      const BlockScale<NV> sc(__float_as_uint(top), p.x_ts);
-      uint32_t w;
-      quantize8<NV>(sc, v[u], &w);
+      for (int o = 1; o < LB; o *= 2) top = absmax(top, __shfl_xor_sync(0xFFFFFFFFu, top, o), 0.0f);
+      const BlockScale<NV> sc(__float_as_uint(top), p.xq);
+      const uint32_t w = quantize8<NV>(sc, v[u]);
       // 128-byte rows, 16-byte pieces swizzled by the row
       *reinterpret_cast<uint32_t *>(codes + (size_t)s * p.NT * 128 + t * 128 + (((lane >> 2) ^ (t & 7)) << 4) + (lane & 3) * 4) = w;
       if (lane % LB == 0)
@@ -1174,7 +1163,7 @@ cudaError_t launch_split(const Fp4Mat &w, const Fp4Mat &xm, const void *x, int x
   p.out_type = out_type;
   p.rot = GLU && a.up_row % 128;
   p.early = early;
-  p.x = x, p.x_type = x_type, p.ldx = ldx, p.x_ts = xm.ts;
+  p.x = x, p.x_type = x_type, p.ldx = ldx, p.xq = xm;
   p.xvec = FUSED && rows_aligned(x, ldx, x_type);
   p.stage = split_stage<NV, GLU, FUSED>(q.NT);
   const uint32_t fixed = (FUSED ? (uint32_t)q.SL * (q.NT * 128 + SC) : 0) +

@@ -61,7 +61,10 @@ t0b_status check_mat(const char *fn, const char *name, const t0b_fp4 *m, bool wr
     if (write && (std::frexp(ts, &ex) != 0.5f || ex - 1 < -64 || ex - 1 > 64))
       return bad(T0B_ERR_INVALID, "needs a power of two in [2^-64, 2^64] as tensor_scale to be quantised into");
   }
-  *out = Fp4Mat{m->codes, m->scales, m->rows, m->k, block_of(m->format), ts};
+  const double r6 = 1.0 / (6.0 * (double)ts);
+  float hi = (float)r6;
+  if ((double)hi > r6) hi = std::nextafter(hi, 0.0f);
+  *out = Fp4Mat{m->codes, m->scales, m->rows, m->k, block_of(m->format), ts, hi, (float)(r6 - (double)hi)};
   return T0B_OK;
 }
 

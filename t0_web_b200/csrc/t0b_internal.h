@@ -133,6 +133,7 @@ struct Fp4Mat {
   uint8_t *codes, *scales;
   int rows, k, blk;
   float ts;
+  float r6_hi, r6_lo;  // 1 / (6 ts) as a sum, hi rounded down (blk 16)
 };
 // Where a product's result goes: y (ggml type `type`, rows ld elements apart)
 // or, for a gated product, the 4-bit matrix q.

@@ -82,9 +82,9 @@ def _plain(engine, name: str, t: torch.Tensor, rows: int, cols: int):
     ty = _TYPES.get(t.dtype)
     if ty is None:
         raise T0bError(T0B_ERR_INVALID, f"fp4: {name} must be float32, float16 or bfloat16, not {t.dtype}")
-    if not t.is_cuda or t.get_device() != engine.device:
+    if t.get_device() != engine.device:  # -1 for host memory
         raise T0bError(T0B_ERR_INVALID, f"fp4: {name} is on {t.device}, the engine on cuda:{engine.device}")
-    if tuple(t.shape) != (rows, cols):
+    if t.shape != (rows, cols):
         raise T0bError(T0B_ERR_INVALID, f"fp4: {name} has shape {tuple(t.shape)}, expected ({rows}, {cols})")
     s0, s1 = t.stride()
     if s1 != 1 and cols > 1:
@@ -95,33 +95,34 @@ def _plain(engine, name: str, t: torch.Tensor, rows: int, cols: int):
 def _bias(engine, name: str, b, n: int):
     if b is None:
         return None
-    if b.dtype != torch.float32 or not b.is_cuda or b.get_device() != engine.device or b.numel() != n or not b.is_contiguous():
+    if b.dtype != torch.float32 or b.get_device() != engine.device or b.numel() != n or not b.is_contiguous():
         raise T0bError(T0B_ERR_INVALID, f"fp4: {name} must be {n} contiguous float32 values on cuda:{engine.device}")
     return b.data_ptr()
 
 
 def _stream(engine, stream):
-    return torch.cuda.current_stream(engine.device).cuda_stream if stream is None else stream
+    # the pointer alone: building torch's Stream object costs more than the rest of a small call's checks
+    return torch._C._cuda_getCurrentRawStream(engine.device) if stream is None else stream
 
 
 def quantize(engine, x: torch.Tensor, out: Fp4Matrix, stream=None) -> Fp4Matrix:
     """x [rows, k] to 4 bits."""
     ty, p, ld = _plain(engine, "x", x, out.rows, out.k)
-    check(lib().t0b_fp4_quantize(engine.handle, ty, p, ld, _mat(engine, out), _stream(engine, stream)))
+    check(lib().t0b_fp4_quantize(engine._h, ty, p, ld, _mat(engine, out), _stream(engine, stream)))
     return out
 
 
 def dequantize(engine, m: Fp4Matrix, y: torch.Tensor, stream=None) -> torch.Tensor:
     """The values of m, rounded to y's type."""
     ty, p, ld = _plain(engine, "y", y, m.rows, m.k)
-    check(lib().t0b_fp4_dequantize(engine.handle, _mat(engine, m), ty, p, ld, _stream(engine, stream)))
+    check(lib().t0b_fp4_dequantize(engine._h, _mat(engine, m), ty, p, ld, _stream(engine, stream)))
     return y
 
 
 def gemm(engine, w: Fp4Matrix, x: Fp4Matrix, y: torch.Tensor, bias=None, stream=None) -> torch.Tensor:
     """y [x.rows, w.rows] = x . w^T (+ bias)."""
     ty, p, ld = _plain(engine, "y", y, x.rows, w.rows)
-    check(lib().t0b_fp4_gemm(engine.handle, _mat(engine, w), _mat(engine, x), _bias(engine, "bias", bias, w.rows), ty, p,
+    check(lib().t0b_fp4_gemm(engine._h, _mat(engine, w), _mat(engine, x), _bias(engine, "bias", bias, w.rows), ty, p,
                              ld, _stream(engine, stream)))
     return y
 
@@ -134,7 +135,7 @@ def glu(engine, w: Fp4Matrix, x: Fp4Matrix, z, bias=None, stream=None):
         ty, p, ld, zq = 0, None, 0, _mat(engine, z)
     else:
         (ty, p, ld), zq = _plain(engine, "z", z, x.rows, w.rows // 2), None
-    check(lib().t0b_fp4_glu(engine.handle, _mat(engine, w), _mat(engine, x), b, ty, p, ld, zq, _stream(engine, stream)))
+    check(lib().t0b_fp4_glu(engine._h, _mat(engine, w), _mat(engine, x), b, ty, p, ld, zq, _stream(engine, stream)))
     return z
 
 
@@ -143,7 +144,7 @@ def linear(engine, w: Fp4Matrix, x: torch.Tensor, xq: Fp4Matrix, y: torch.Tensor
     afterwards are unspecified) and the product in one call."""
     xt, xp, xld = _plain(engine, "x", x, xq.rows, xq.k)
     ty, p, ld = _plain(engine, "y", y, xq.rows, w.rows)
-    check(lib().t0b_fp4_linear(engine.handle, _mat(engine, w), xt, xp, xld, _mat(engine, xq),
+    check(lib().t0b_fp4_linear(engine._h, _mat(engine, w), xt, xp, xld, _mat(engine, xq),
                                _bias(engine, "bias", bias, w.rows), ty, p, ld, _stream(engine, stream)))
     return y
 
@@ -154,7 +155,7 @@ def mlp(engine, w0: Fp4Matrix, w2: Fp4Matrix, x: torch.Tensor, xq: Fp4Matrix, zq
     (the contents of xq and zq afterwards are unspecified)."""
     xt, xp, xld = _plain(engine, "x", x, xq.rows, xq.k)
     ty, p, ld = _plain(engine, "y", y, xq.rows, w2.rows)
-    check(lib().t0b_fp4_mlp(engine.handle, _mat(engine, w0), _mat(engine, w2), xt, xp, xld, _mat(engine, xq),
+    check(lib().t0b_fp4_mlp(engine._h, _mat(engine, w0), _mat(engine, w2), xt, xp, xld, _mat(engine, xq),
                             _mat(engine, zq), _bias(engine, "b0", b0, w0.rows), _bias(engine, "b2", b2, w2.rows), ty, p,
                             ld, _stream(engine, stream)))
     return y
@@ -162,4 +163,4 @@ def mlp(engine, w0: Fp4Matrix, w2: Fp4Matrix, x: torch.Tensor, xq: Fp4Matrix, zq
 
 def sync(engine, stream=None) -> None:
     """Wait for the stream and raise any kernel-side error of the engine's 4-bit operators."""
-    check(lib().t0b_fp4_sync(engine.handle, _stream(engine, stream)))
+    check(lib().t0b_fp4_sync(engine._h, _stream(engine, stream)))
