@@ -81,6 +81,24 @@ T0B_DEV void values8(uint32_t w, float *v) {
   }
 }
 
+// Pairs of f32, two lanes of one instruction.
+struct F2 {
+  uint64_t v;
+  T0B_DEV F2(uint64_t x) : v(x) {}
+  T0B_DEV F2(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
+  T0B_DEV void get(float &a, float &b) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+};
+T0B_DEV F2 fma2(F2 a, F2 b, F2 c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return d;
+}
+T0B_DEV F2 mul2(F2 a, F2 b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a.v), "l"(b.v));
+  return d;
+}
+
 // The largest of a and two magnitudes; keeps a NaN (as bits above infinity's).
 T0B_DEV float absmax(float a, float b, float c) {
   float r;
@@ -122,10 +140,6 @@ struct BlockScale {
       lo = fmaf(-hi, d, 1.0f) * hi;
     }
   }
-  T0B_DEV float quotient(float x) const {
-    if constexpr (!NV) return x * hi;
-    return fmaf(x, hi, x * lo);
-  }
 };
 
 // Eight values of a block to a word of codes.
@@ -133,7 +147,13 @@ template <bool NV>
 T0B_DEV uint32_t quantize8(const BlockScale<NV> &s, const float *v) {
   float u[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) u[j] = s.quotient(v[j]);
+  for (int j = 0; j < 8; j += 2) {
+    const F2 x(v[j], v[j + 1]), hi(s.hi, s.hi);
+    if constexpr (NV)
+      fma2(x, hi, mul2(x, F2(s.lo, s.lo))).get(u[j], u[j + 1]);
+    else
+      mul2(x, hi).get(u[j], u[j + 1]);
+  }
   const uint32_t w = codes8(u);
   return NV && s.byte == 0 ? 0u : w;  // a scale of zero: no signs either
 }
@@ -146,55 +166,79 @@ T0B_DEV uint32_t quantize8(const BlockScale<NV> &s, const float *v) {
 // two (NV) or four lanes; its largest magnitude and the tile's scale words are
 // joined by shuffles.
 constexpr int QT_WARPS = 8;
+constexpr int QT_CHUNKS = 4;  // 65,536 x 1024 bf16: 39 us with 1, 35 with 2, 32 with 4 and 8
 
-// 8 values from x[k0 ..], zeros from k on; `vec`: rows are 16-byte aligned.
+// 8 values from x[k0 ..] as they lie in memory, zeros from k on; `vec`: rows
+// are 16-byte aligned.
 template <int TY>
-T0B_DEV void load8(const typename Plain<TY>::T *x, int k0, int k, bool vec, float *v) {
+struct Raw8 {
   using T = typename Plain<TY>::T;
-  if (vec && k0 + 8 <= k) {
-    uint4 t[sizeof(T) / 2];
+  uint4 w[sizeof(T) / 2];
+  T0B_DEV void load(const T *x, int k0, int k, bool vec) {
+    if (vec && k0 + 8 <= k) {
 #pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; ++i) t[i] = reinterpret_cast<const uint4 *>(x + k0)[i];
-    const T *e = reinterpret_cast<const T *>(t);
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = reinterpret_cast<const uint4 *>(x + k0)[i];
+    } else {
+      T e[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) e[i] = k0 + i < k ? x[k0 + i] : Plain<TY>::put(0.0f);
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = reinterpret_cast<const uint4 *>(e)[i];
+    }
+  }
+  T0B_DEV void zero() {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = make_uint4(0, 0, 0, 0);
+  }
+  T0B_DEV void get(float *v) const {
+    const T *e = reinterpret_cast<const T *>(w);
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = Plain<TY>::get(e[i]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = k0 + i < k ? Plain<TY>::get(x[k0 + i]) : 0.0f;
   }
-}
+};
 
 // LPR: lanes along a row, a scale tile's (8 or 16) or 32.
+// A warp goes through `chunks` such pieces along its rows and fetches the next
+// one before it works on the present one.
 template <int TY, bool NV, int LPR>
-__global__ void __launch_bounds__(32 * QT_WARPS) fp4_quantize_kernel(const typename Plain<TY>::T *x, int64_t ldx, Fp4Mat q, bool vec) {
+__global__ void __launch_bounds__(32 * QT_WARPS)
+    fp4_quantize_kernel(const typename Plain<TY>::T *x, int64_t ldx, Fp4Mat q, bool vec, int chunks) {
   constexpr int BLK = NV ? 16 : 32, LB = BLK / 8;  // lanes of a block
   constexpr int RPW = 32 / LPR;                    // adjacent rows of a warp
   const int kt = (q.k + 4 * BLK - 1) / (4 * BLK);
   const int lane = threadIdx.x & 31;
   const int r0 = blockIdx.x * (QT_WARPS * RPW) + (threadIdx.x >> 5) * RPW + lane / LPR;  // counts 32 rows of each group
   const int group = r0 >> 5, r = group * 128 + (r0 & 31);
-  const int k0 = (blockIdx.y * LPR + lane % LPR) * 8;
+  int k0 = (blockIdx.y * chunks * LPR + lane % LPR) * 8;
   pdl_wait();
   pdl_launch_dependents();
-  float v[4][8];
+  Raw8<TY> next[4];
+  auto fetch = [&](int k) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (r + 32 * i < q.rows)
-      load8<TY>(x + (r + 32 * i) * ldx, k0, q.k, vec, v[i]);
-    else
+    for (int i = 0; i < 4; ++i)
+      if (r + 32 * i < q.rows)
+        next[i].load(x + (r + 32 * i) * ldx, k, q.k, vec);
+      else
+        next[i].zero();
+  };
+  fetch(k0);
+  for (int c = 0; c < chunks; ++c, k0 += 8 * LPR) {
+  Raw8<TY> raw[4];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[i][j] = 0.0f;
-  }
+  for (int i = 0; i < 4; ++i) raw[i] = next[i];
+  if (c + 1 < chunks) fetch(k0 + 8 * LPR);
   uint32_t sc = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    float top = absmax_of<8>(v[i]);
+    float v[8];
+    raw[i].get(v);
+    float top = absmax_of<8>(v);
 #pragma unroll
     for (int o = 1; o < LB; o *= 2) top = absmax(top, __shfl_xor_sync(0xFFFFFFFFu, top, o), 0.0f);
     const BlockScale<NV> s(__float_as_uint(top), q);
     sc |= s.byte << (8 * i);
     if (r + 32 * i < q.rows && k0 / 2 < (int)code_pitch(q.k))
-      *reinterpret_cast<uint32_t *>(q.codes + (r + 32 * i) * code_pitch(q.k) + k0 / 2) = quantize8<NV>(s, v[i]);
+      *reinterpret_cast<uint32_t *>(q.codes + (r + 32 * i) * code_pitch(q.k) + k0 / 2) = quantize8<NV>(s, v);
   }
   // sc: one block of four rows; the tile's words are four blocks of one row
   const int b = lane / LB % 4;
@@ -203,6 +247,7 @@ __global__ void __launch_bounds__(32 * QT_WARPS) fp4_quantize_kernel(const typen
   const int t = k0 / (4 * BLK);
   if (lane % LB == 0 && t < kt && group < (q.rows + 127) / 128)
     *reinterpret_cast<uint32_t *>(q.scales + ((size_t)group * kt + t) * 512 + (r & 31) * 16 + 4 * b) = sc;
+  }
 }
 
 // ----------------------------------------------------------- the other way
@@ -254,20 +299,37 @@ __global__ void __launch_bounds__(32 * QT_WARPS) fp4_dequantize_kernel(Fp4Mat q,
 }
 
 // ----------------------------------------------------------------- product
-// silu(g) * u.  1 / (1 + exp(-g)) with exp as 2^t, t = -g log2(e) carried to
+// silu(g) * u.  1 / (1 + exp(-g)) with exp as 2^-t, t = g log2(e) carried to
 // twice the precision (the rounding error of t would otherwise grow with g);
-// g is clamped where the sigmoid is 0 or 1 to the last bit.
-T0B_DEV float silu_mul(float g, float u) {
-  constexpr float L = 1.44269504f, L2 = 1.92596299e-8f, LN2 = 0.693147181f;
-  const float c = fminf(fmaxf(g, -126.0f), 126.0f);
-  const float t = -c * L;
-  const float e = fmaf(-c, L2, fmaf(-c, L, -t));  // the part of -c log2(e) that t lost
+// beyond +-126 the sigmoid is 0 or 1 to the last bit, and the clamp keeps the
+// correction finite.
+constexpr float LOG2E = 1.44269504f, LOG2E_LO = 1.92596299e-8f, LN2 = 0.693147181f;
+T0B_DEV float ex2_neg(float t) {
   float p;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p) : "f"(t));
-  p *= fmaf(e, LN2, 1.0f);
-  float s;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(1.0f + p));
-  return g * s * u;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p) : "f"(-t));
+  return p;
+}
+T0B_DEV float rcp_approx(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+T0B_DEV float silu_mul(float g, float u) {
+  const float c = fminf(fmaxf(g, -126.0f), 126.0f);
+  const float t = __fmul_rn(c, LOG2E);
+  const float f = fmaf(fmaf(c, -LOG2E_LO, fmaf(c, -LOG2E, t)), LN2, 1.0f);
+  return __fmul_rn(__fmul_rn(g, rcp_approx(fmaf(ex2_neg(t), f, 1.0f))), u);
+}
+// The same on pairs, for |g| below 2^20 (no clamp: the correction stays near 1
+// there), with the same results.
+T0B_DEV F2 silu_mul2(F2 g, F2 u) {
+  const F2 t = mul2(g, F2(LOG2E, LOG2E));
+  const F2 e = fma2(g, F2(-LOG2E_LO, -LOG2E_LO), fma2(g, F2(-LOG2E, -LOG2E), t));
+  const F2 f = fma2(e, F2(LN2, LN2), F2(1.0f, 1.0f));
+  float t0, t1, d0, d1;
+  t.get(t0, t1);
+  fma2(F2(ex2_neg(t0), ex2_neg(t1)), f, F2(1.0f, 1.0f)).get(d0, d1);
+  return mul2(mul2(g, F2(rcp_approx(d0), rcp_approx(d1))), u);
 }
 
 // 32 accumulator columns of this thread's lane; the values may be used after
@@ -657,11 +719,24 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
         }
       } else {
         const int c0 = 32 * h, f0 = nt * 128 + c0;
-        float v[32];
+        const F2 alpha(p.alpha, p.alpha);
+        float *g = reinterpret_cast<float *>(r[0]), *u = reinterpret_cast<float *>(r[1]), *v = g;
+        const float4 *bg = reinterpret_cast<const float4 *>(sbias + c0), *bu = reinterpret_cast<const float4 *>(sbias + 128 + c0);
 #pragma unroll
-        for (int j = 0; j < 32; ++j)
-          v[j] = silu_mul(fmaf(__uint_as_float(r[0][j]), p.alpha, sbias[c0 + j]),
-                          fmaf(__uint_as_float(r[1][j]), p.alpha, sbias[128 + c0 + j]));
+        for (int j = 0; j < 32; j += 4) {
+          const float4 b = bg[j / 4], d = bu[j / 4];
+          fma2(F2(g[j], g[j + 1]), alpha, F2(b.x, b.y)).get(g[j], g[j + 1]);
+          fma2(F2(g[j + 2], g[j + 3]), alpha, F2(b.z, b.w)).get(g[j + 2], g[j + 3]);
+          fma2(F2(u[j], u[j + 1]), alpha, F2(d.x, d.y)).get(u[j], u[j + 1]);
+          fma2(F2(u[j + 2], u[j + 3]), alpha, F2(d.z, d.w)).get(u[j + 2], u[j + 3]);
+        }
+        if (absmax_of<32>(g) < 1048576.0f) {
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) silu_mul2(F2(g[j], g[j + 1]), F2(u[j], u[j + 1])).get(v[j], v[j + 1]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = silu_mul(g[j], u[j]);
+        }
         if constexpr (TY >= 0) {
 #pragma unroll
           for (int i = 0; i < 32 / W; ++i) store_rows<OT>(p, &tm_y, stg, row0, f0 + W * i, v + W * i);
@@ -799,22 +874,24 @@ T0B_DEV void quantize_slice(const SplitArgs &p, uint8_t *codes, uint8_t *scales,
   const auto *x = reinterpret_cast<const typename Plain<TY>::T *>(p.x);
   const int n = toks * stages;
   for (int i0 = warp; i0 < n; i0 += U * (SPLIT_THREADS / 32)) {
-    float v[U][8];
+    Raw8<TY> raw[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int i = i0 + u * (SPLIT_THREADS / 32);
-      if (i < n) load8<TY>(x + (int64_t)(m0 + i / stages) * p.ldx, k_begin + i % stages * 256 + lane * 8, p.a.K, p.xvec, v[u]);
+      if (i < n) raw[u].load(x + (int64_t)(m0 + i / stages) * p.ldx, k_begin + i % stages * 256 + lane * 8, p.a.K, p.xvec);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int i = i0 + u * (SPLIT_THREADS / 32);
       if (i >= n) break;
       const int t = i / stages, s = i % stages;
-      float top = absmax_of<8>(v[u]);
+      float v[8];
+      raw[u].get(v);
+      float top = absmax_of<8>(v);
 #pragma unroll
       for (int o = 1; o < LB; o *= 2) top = absmax(top, __shfl_xor_sync(0xFFFFFFFFu, top, o), 0.0f);
       const BlockScale<NV> sc(__float_as_uint(top), p.xq);
-      const uint32_t w = quantize8<NV>(sc, v[u]);
+      const uint32_t w = quantize8<NV>(sc, v);
       // 128-byte rows, 16-byte pieces swizzled by the row
       *reinterpret_cast<uint32_t *>(codes + (size_t)s * p.NT * 128 + t * 128 + (((lane >> 2) ^ (t & 7)) << 4) + (lane & 3) * 4) = w;
       if (lane % LB == 0)
@@ -1126,16 +1203,17 @@ int max_pairs(const void *kfn, const cudaLaunchConfig_t &cfg) {
 
 bool rows_aligned(const void *p, int64_t ld, int type) { return ((uintptr_t)p | (uint64_t)ld * (type == TY_F32 ? 4 : 2)) % 16 == 0; }
 
-// How a product is divided for the split kernel.
-struct SplitPlan {
-  int NT, CS, SL, rt;
-  int64_t ctas;
-};
 int sm_count() {
   int dev = 0, n = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
   return n;
 }
+
+// How a product is divided for the split kernel.
+struct SplitPlan {
+  int NT, CS, SL, rt;
+  int64_t ctas;
+};
 SplitPlan split_plan(bool glu, int M, int n, int K, int sms) {
   SplitPlan q;
   const int most = glu ? 64 : 128;  // tokens of a tile; several tiles start at whole scale columns
@@ -1272,11 +1350,14 @@ cudaError_t convert(const void *x, int64_t ld, const Fp4Mat &q, cudaStream_t st)
   const bool vec = rows_aligned(x, ld, TY), narrow = q.k <= 8 * SHORT;
   const int lpr = narrow ? SHORT : 32, row_warps = (q.rows + 127) / 128 * lpr;  // of 32 / lpr rows, 32 rows a group
   const int width = QUANT ? (q.k + 8 * SHORT - 1) / (8 * SHORT) * (8 * SHORT) : q.k;  // whole scale tiles
-  const dim3 grid((row_warps + QT_WARPS - 1) / QT_WARPS, (width + 8 * lpr - 1) / (8 * lpr));
-  if constexpr (QUANT)
-    return narrow ? launch(fp4_quantize_kernel<TY, NV, SHORT>, grid, 32 * QT_WARPS, st, (const T *)x, ld, q, vec)
-                  : launch(fp4_quantize_kernel<TY, NV, 32>, grid, 32 * QT_WARPS, st, (const T *)x, ld, q, vec);
-  else
+  dim3 grid((row_warps + QT_WARPS - 1) / QT_WARPS, (width + 8 * lpr - 1) / (8 * lpr));
+  if constexpr (QUANT) {
+    // pieces of a row one after the other in a warp, as long as two waves of CTAs remain
+    int chunks = 1;
+    while (chunks < QT_CHUNKS && grid.y > 1 && (int64_t)grid.x * grid.y > 2 * 4 * sm_count()) chunks *= 2, grid.y = (grid.y + 1) / 2;
+    return narrow ? launch(fp4_quantize_kernel<TY, NV, SHORT>, grid, 32 * QT_WARPS, st, (const T *)x, ld, q, vec, chunks)
+                  : launch(fp4_quantize_kernel<TY, NV, 32>, grid, 32 * QT_WARPS, st, (const T *)x, ld, q, vec, chunks);
+  } else
     return narrow ? launch(fp4_dequantize_kernel<TY, NV, SHORT>, grid, 32 * QT_WARPS, st, q, (T *)x, ld, vec)
                   : launch(fp4_dequantize_kernel<TY, NV, 32>, grid, 32 * QT_WARPS, st, q, (T *)x, ld, vec);
 }
