@@ -445,11 +445,13 @@ struct PairCfg {
   static constexpr int NS = NV && ROT ? 4 : 5;             // stages
   static constexpr uint32_t OFF_A = 0, OFF_B = CODES, OFF_SA = 2 * CODES, OFF_SB = OFF_SA + SC, OFF_RAW = OFF_SB + 2 * SC;
   static constexpr uint32_t OFF_STG = NS * STAGE;          // 32 rows x 64 bytes per epilogue warp
-  static constexpr uint32_t OFF_BIAS = OFF_STG + PAIR_EPI_WARPS * 2048, OFF_BAR = OFF_BIAS + 256 * 4;
-  static constexpr uint32_t SMEM = OFF_BAR + 256 + 1024;
+  static constexpr uint32_t OFF_BIAS = OFF_STG + PAIR_EPI_WARPS * 2048;  // 64 floats per epilogue warp
+  static constexpr uint32_t OFF_BAR = OFF_BIAS + PAIR_EPI_WARPS * 256, USED = OFF_BAR + 256;
+  // and up to 1024 bytes to align the start, which is aligned already as far as it goes
+  static constexpr uint32_t SMEM = USED + 1024 < 232448 ? USED + 1024 : 232448;
   static constexpr uint32_t SFC = AT * 12;                 // TMEM columns of a stage's scales
   static_assert(256 + NS * SFC <= 512, "accumulator and scales in TMEM");
-  static_assert(STAGE % 1024 == 0 && SMEM <= 232448, "shared memory");
+  static_assert(STAGE % 1024 == 0 && USED <= 232448, "shared memory");
 };
 
 // 32 consecutive values of row r, columns c0 .. (a multiple of 32), to 4 bits;
@@ -530,7 +532,7 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t *smem = smem_raw + (base - smem_u32(smem_raw));
-  if (cluster_size() != 2) {
+  if (cluster_size() != 2 || base - smem_u32(smem_raw) > C::SMEM - C::USED) {
     if (threadIdx.x == 0) record_error(p.err, T0B_DEVERR_SHAPE);
     return;
   }
@@ -544,7 +546,6 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
   uint64_t *mma_done = acc_empty + 1;
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(mma_done + 1);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(mma_done + 2);
-  float *sbias = reinterpret_cast<float *>(smem + C::OFF_BIAS);
   const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int S = (p.K + 255) / 256;
   const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
@@ -680,17 +681,19 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
     // ------------------------------------------------------------ epilogue (both CTAs)
     setmaxnreg_inc<PAIR_REGS_EPI>();
     const int q = warp & 3, h = (warp - 4) >> 2;  // lane quarter, 64 columns (gated: 32 gate, 32 up)
-    const int et = threadIdx.x - 128;
     uint8_t *stg = smem + C::OFF_STG + (warp - 4) * 2048;
+    float *sb = reinterpret_cast<float *>(smem + C::OFF_BIAS) + (warp - 4) * 64;
     uint32_t it = 0;
     for (int tile = pair; tile < p.n_tiles; tile += npairs, ++it) {
       const int nt = tile % p.n_tiles_n, m0 = tile / p.n_tiles_n * 256 + 128 * (int)rank;
-      asm volatile("bar.sync 1, 512;" ::: "memory");
-      if (et < 256) {
-        const int col = GLU ? nt * 128 + (et & 127) : nt * 256 + et;
-        sbias[et] = p.bias && col < p.n ? p.bias[GLU && et >= 128 ? p.n + col : col] : 0.0f;
+      // this warp's 64 biases (gated: 32 gate, 32 up)
+      __syncwarp();
+      {
+        const int c0 = GLU ? nt * 128 + 32 * h + lane : nt * 256 + 64 * h + lane, c1 = GLU ? c0 : c0 + 32;
+        sb[lane] = p.bias && c0 < p.n ? p.bias[c0] : 0.0f;
+        sb[32 + lane] = p.bias && c1 < p.n ? p.bias[GLU ? p.n + c1 : c1] : 0.0f;
       }
-      asm volatile("bar.sync 1, 512;" ::: "memory");
+      __syncwarp();
       const int row0 = m0 + 32 * q;
       const uint32_t trow = tmem + ((uint32_t)(32 * q) << 16);
       bool have = mbar_wait(acc_full, it & 1, p.err, T0B_DEVERR_WAIT_ACC, abort_flag) && !*abort_flag;
@@ -714,17 +717,23 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
           const int c0 = 64 * h + W * i;
           float v[W];
 #pragma unroll
-          for (int j = 0; j < W; ++j) v[j] = fmaf(__uint_as_float(r[i * W / 32][i * W % 32 + j]), p.alpha, sbias[c0 + j]);
+          for (int j = 0; j < W; j += 4) {
+            const float4 b = *reinterpret_cast<const float4 *>(sb + W * i + j);
+            const uint32_t *a = r[i * W / 32] + i * W % 32 + j;
+            v[j] = fmaf(__uint_as_float(a[0]), p.alpha, b.x);
+            v[j + 1] = fmaf(__uint_as_float(a[1]), p.alpha, b.y);
+            v[j + 2] = fmaf(__uint_as_float(a[2]), p.alpha, b.z);
+            v[j + 3] = fmaf(__uint_as_float(a[3]), p.alpha, b.w);
+          }
           store_rows<OT>(p, &tm_y, stg, row0, nt * 256 + c0, v);
         }
       } else {
         const int c0 = 32 * h, f0 = nt * 128 + c0;
         const F2 alpha(p.alpha, p.alpha);
         float *g = reinterpret_cast<float *>(r[0]), *u = reinterpret_cast<float *>(r[1]), *v = g;
-        const float4 *bg = reinterpret_cast<const float4 *>(sbias + c0), *bu = reinterpret_cast<const float4 *>(sbias + 128 + c0);
 #pragma unroll
         for (int j = 0; j < 32; j += 4) {
-          const float4 b = bg[j / 4], d = bu[j / 4];
+          const float4 b = *reinterpret_cast<const float4 *>(sb + j), d = *reinterpret_cast<const float4 *>(sb + 32 + j);
           fma2(F2(g[j], g[j + 1]), alpha, F2(b.x, b.y)).get(g[j], g[j + 1]);
           fma2(F2(g[j + 2], g[j + 3]), alpha, F2(b.z, b.w)).get(g[j + 2], g[j + 3]);
           fma2(F2(u[j], u[j + 1]), alpha, F2(d.x, d.y)).get(u[j], u[j + 1]);
