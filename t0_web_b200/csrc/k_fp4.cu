@@ -252,7 +252,9 @@ __global__ void __launch_bounds__(32 * QT_WARPS)
 
 // ----------------------------------------------------------- the other way
 // The same division of work: 4 bytes of codes to 8 values a lane, the scale
-// words of four rows in one 16-byte load.
+// words of four rows in one 16-byte load.  8 values of a lane go out at once
+// where rows are aligned to them (the largest: 32 bytes, so that no sector is
+// written in halves).
 template <int TY>
 T0B_DEV void store8(typename Plain<TY>::T *y, int k0, int k, bool vec, const float *v) {
   using T = typename Plain<TY>::T;
@@ -260,12 +262,47 @@ T0B_DEV void store8(typename Plain<TY>::T *y, int k0, int k, bool vec, const flo
 #pragma unroll
   for (int i = 0; i < 8; ++i) t[i] = Plain<TY>::put(v[i]);
   if (vec && k0 + 8 <= k) {
-#pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4 *>(y + k0)[i] = reinterpret_cast<const uint4 *>(t)[i];
+    if constexpr (TY == TY_F32)
+      asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(y + k0), "f"(v[0]), "f"(v[1]), "f"(v[2]),
+                   "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
+                   : "memory");
+    else
+      *reinterpret_cast<uint4 *>(y + k0) = *reinterpret_cast<const uint4 *>(t);
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
       if (k0 + i < k) y[k0 + i] = t[i];
+  }
+}
+// A warp's 256 values of a row that is not aligned, columns c0 .. of k, turned
+// in shared memory so that the lanes write neighbouring 4-byte words (two
+// 16-bit values; single ones at the ends).
+template <int TY>
+T0B_DEV void store_unaligned(typename Plain<TY>::T *y, int c0, int k, typename Plain<TY>::T *sm, const float *v) {
+  using T = typename Plain<TY>::T;
+  const int lane = threadIdx.x & 31, n = min(256, k - c0);
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) sm[lane * 8 + i] = Plain<TY>::put(v[i]);
+  __syncwarp();
+  y += c0;
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (lane + 32 * i < n) y[lane + 32 * i] = sm[lane + 32 * i];
+  } else {
+    const int odd = (int)((uintptr_t)y >> 1 & 1);
+#pragma unroll
+    for (int i = 0; i < 5; ++i) {
+      const int e = 2 * (lane + 32 * i) - odd;  // values e, e + 1 share a word
+      if (e >= n || e > 255) break;
+      if (e >= 0 && e + 1 < n) {
+        const T t[2] = {sm[e], sm[e + 1]};
+        *reinterpret_cast<uint32_t *>(y + e) = *reinterpret_cast<const uint32_t *>(t);
+      } else {
+        y[e < 0 ? 0 : e] = sm[e < 0 ? 0 : e];
+      }
+    }
   }
 }
 
@@ -279,13 +316,18 @@ __global__ void __launch_bounds__(32 * QT_WARPS) fp4_dequantize_kernel(Fp4Mat q,
   const int k0 = (blockIdx.y * LPR + lane % LPR) * 8;
   pdl_wait();
   pdl_launch_dependents();
-  if (k0 >= q.k || r >= q.rows) return;
-  const uint4 s4 = *reinterpret_cast<const uint4 *>(q.scales + ((size_t)group * kt + k0 / (4 * BLK)) * 512 + (r & 31) * 16);
+  // rows that are not aligned are written by the whole warp
+  const bool turn = LPR == 32 && !vec;
+  if ((k0 >= q.k && !turn) || r >= q.rows) return;
+  __shared__ typename Plain<TY>::T turned[QT_WARPS][LPR == 32 ? 256 : 1];
+  const bool in = k0 < q.k;
+  uint4 s4 = make_uint4(0, 0, 0, 0);
+  if (in) s4 = *reinterpret_cast<const uint4 *>(q.scales + ((size_t)group * kt + k0 / (4 * BLK)) * 512 + (r & 31) * 16);
   const uint32_t sw[4] = {s4.x, s4.y, s4.z, s4.w};
-  uint32_t w[4];
+  uint32_t w[4] = {};
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    if (r + 32 * i < q.rows) w[i] = *reinterpret_cast<const uint32_t *>(q.codes + (r + 32 * i) * code_pitch(q.k) + k0 / 2);
+    if (r + 32 * i < q.rows && in) w[i] = *reinterpret_cast<const uint32_t *>(q.codes + (r + 32 * i) * code_pitch(q.k) + k0 / 2);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     if (r + 32 * i >= q.rows) break;
@@ -294,7 +336,10 @@ __global__ void __launch_bounds__(32 * QT_WARPS) fp4_dequantize_kernel(Fp4Mat q,
     values8(w[i], v);
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = NV ? v[j] * s * q.ts : v[j] * s;
-    store8<TY>(y + (r + 32 * i) * ldy, k0, q.k, vec, v);
+    if (turn)
+      store_unaligned<TY>(y + (r + 32 * i) * ldy, blockIdx.y * 256, q.k, turned[threadIdx.x >> 5], v);
+    else
+      store8<TY>(y + (r + 32 * i) * ldy, k0, q.k, vec, v);
   }
 }
 
@@ -1356,7 +1401,8 @@ template <int TY, bool NV, bool QUANT>
 cudaError_t convert(const void *x, int64_t ld, const Fp4Mat &q, cudaStream_t st) {
   using T = typename Plain<TY>::T;
   constexpr int SHORT = NV ? 8 : 16;
-  const bool vec = rows_aligned(x, ld, TY), narrow = q.k <= 8 * SHORT;
+  // expansion writes 32 bytes of f32 at once
+  const bool vec = QUANT || TY != TY_F32 ? rows_aligned(x, ld, TY) : ((uintptr_t)x | (uint64_t)ld * 4) % 32 == 0, narrow = q.k <= 8 * SHORT;
   const int lpr = narrow ? SHORT : 32, row_warps = (q.rows + 127) / 128 * lpr;  // of 32 / lpr rows, 32 rows a group
   const int width = QUANT ? (q.k + 8 * SHORT - 1) / (8 * SHORT) * (8 * SHORT) : q.k;  // whole scale tiles
   dim3 grid((row_warps + QT_WARPS - 1) / QT_WARPS, (width + 8 * lpr - 1) / (8 * lpr));
