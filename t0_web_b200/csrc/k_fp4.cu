@@ -556,13 +556,31 @@ T0B_DEV void store_rows(const Fp4Args &p, const void *tm_y, uint8_t *stg, int ro
     }
   } else {
     __syncwarp();
-    T *y = reinterpret_cast<T *>(p.y);
-    const int c = lane % W;
+    // half a warp a row, 4-byte words: 16-bit values in pairs, single ones at the ends
+    auto at = [&](int r, int c) {
+      return *reinterpret_cast<const T *>(stg + r * 64 + (((c * (int)sizeof(T) >> 4) ^ ((r >> 1) & 3)) << 4) + (c * (int)sizeof(T) & 15));
+    };
+    const int n = min(W, p.n - c0), hl = lane & 15;
+    T *y = reinterpret_cast<T *>(p.y) + (int64_t)(row0 + (lane >> 4)) * p.ld + c0;
 #pragma unroll 4
-    for (int r = lane / W; r < 32; r += 32 / W)
-      if (row0 + r < p.M && c0 + c < p.n)
-        y[(row0 + r) * p.ld + c0 + c] =
-            *reinterpret_cast<const T *>(stg + r * 64 + (((c * (int)sizeof(T) >> 4) ^ ((r >> 1) & 3)) << 4) + (c * (int)sizeof(T) & 15));
+    for (int r = lane >> 4; r < 32; r += 2, y += 2 * p.ld) {
+      if (row0 + r >= p.M) break;
+      if constexpr (sizeof(T) == 4) {
+        if (hl < n) y[hl] = at(r, hl);
+      } else {
+        const int e = 2 * hl - (int)((uintptr_t)y >> 1 & 1);
+        if (e >= 0 && e + 1 < n) {
+          const T t[2] = {at(r, e), at(r, e + 1)};
+          *reinterpret_cast<uint32_t *>(y + e) = *reinterpret_cast<const uint32_t *>(t);
+        } else if (e < n) {
+          y[e < 0 ? 0 : e] = at(r, e < 0 ? 0 : e);
+        }
+      }
+    }
+    if constexpr (sizeof(T) == 2) {  // the last value of rows that start in the middle of a word, one row a lane
+      y = reinterpret_cast<T *>(p.y) + (int64_t)(row0 + lane) * p.ld + c0;
+      if (n == W && row0 + lane < p.M && ((uintptr_t)y >> 1 & 1)) y[W - 1] = at(lane, W - 1);
+    }
   }
 }
 
