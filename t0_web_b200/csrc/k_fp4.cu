@@ -561,6 +561,7 @@ T0B_DEV void store_rows(const Fp4Args &p, const void *tm_y, uint8_t *stg, int ro
       return *reinterpret_cast<const T *>(stg + r * 64 + (((c * (int)sizeof(T) >> 4) ^ ((r >> 1) & 3)) << 4) + (c * (int)sizeof(T) & 15));
     };
     const int n = min(W, p.n - c0), hl = lane & 15;
+    if (n <= 0) return;
     T *y = reinterpret_cast<T *>(p.y) + (int64_t)(row0 + (lane >> 4)) * p.ld + c0;
 #pragma unroll 4
     for (int r = lane >> 4; r < 32; r += 2, y += 2 * p.ld) {
@@ -861,15 +862,6 @@ struct SplitArgs {
   int xvec;
 };
 
-T0B_DEV void store_elem(void *y, int type, int64_t i, float v) {
-  if (type == TY_F32)
-    reinterpret_cast<float *>(y)[i] = v;
-  else if (type == TY_F16)
-    reinterpret_cast<__half *>(y)[i] = __float2half_rn(v);
-  else
-    reinterpret_cast<__nv_bfloat16 *>(y)[i] = __float2bfloat16_rn(v);
-}
-
 // One value per lane, 32 consecutive columns c0 .. c0 + 31 of row r (zeros
 // behind the matrix) to 4 bits.  Every lane of the warp calls it; c0 is a
 // multiple of 32.  Rows behind the matrix get zero scales.
@@ -892,15 +884,19 @@ T0B_DEV void quantize_lanes(const Fp4Mat &q, int r, int c0, float v) {
     *reinterpret_cast<uint32_t *>(q.codes + r * code_pitch(q.k) + (c0 + lane) / 2) = w;
 }
 
-T0B_DEV void tmem_ld8(uint32_t addr, float *v) {
-  uint32_t r[8];
+// 16 accumulator columns of this thread's lane; used after the wait on them.
+T0B_DEV void tmem_ld16(uint32_t addr, uint32_t *r) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n tcgen05.wait::ld.sync.aligned;"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
-      : "r"(addr)
-      : "memory");
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[i]);
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(addr));
+}
+T0B_DEV void tmem_ld_wait16(uint32_t *r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]),
+                 "+r"(r[15])::"memory");
 }
 T0B_DEV void scale_cp(uint32_t taddr, uint64_t desc) {
   asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
@@ -940,36 +936,135 @@ __host__ __device__ constexpr uint32_t split_stage(int NT) {
 
 template <int TY, bool NV>
 T0B_DEV void quantize_slice(const SplitArgs &p, uint8_t *codes, uint8_t *scales, int m0, int toks, int k_begin, int stages) {
-  // a warp takes 256 values (a stage) of a token; four at a time
-  constexpr int AT = NV ? 4 : 2, BLK = NV ? 16 : 32, LB = BLK / 8, U = 4;
+  // a warp takes 256 values (a stage) of a token, four such pieces at a time,
+  // the next four on their way meanwhile
+  constexpr int AT = NV ? 4 : 2, BLK = NV ? 16 : 32, LB = BLK / 8, U = 4, W = SPLIT_THREADS / 32;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const auto *x = reinterpret_cast<const typename Plain<TY>::T *>(p.x);
   const int n = toks * stages;
-  for (int i0 = warp; i0 < n; i0 += U * (SPLIT_THREADS / 32)) {
+  const uint32_t inv = (65536u + (uint32_t)stages - 1) / (uint32_t)stages;  // i / stages for i < 4096, stages <= 8
+  auto token = [&](int i) { return (int)((uint32_t)i * inv >> 16); };
+  Raw8<TY> next[U];
+  auto fetch = [&](int i0) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * W, t = token(i);
+      if (i < n) next[u].load(x + (int64_t)(m0 + t) * p.ldx, k_begin + (i - t * stages) * 256 + lane * 8, p.a.K, p.xvec);
+    }
+  };
+  fetch(warp);
+  for (int i0 = warp; i0 < n; i0 += U * W) {
     Raw8<TY> raw[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int i = i0 + u * (SPLIT_THREADS / 32);
-      if (i < n) raw[u].load(x + (int64_t)(m0 + i / stages) * p.ldx, k_begin + i % stages * 256 + lane * 8, p.a.K, p.xvec);
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int i = i0 + u * (SPLIT_THREADS / 32);
-      if (i >= n) break;
-      const int t = i / stages, s = i % stages;
+    for (int u = 0; u < U; ++u) raw[u] = next[u];
+    fetch(i0 + U * W);
+    auto piece = [&](int u) {
+      const int i = i0 + u * W, t = token(i), s = i - t * stages;
       float v[8];
       raw[u].get(v);
       float top = absmax_of<8>(v);
 #pragma unroll
       for (int o = 1; o < LB; o *= 2) top = absmax(top, __shfl_xor_sync(0xFFFFFFFFu, top, o), 0.0f);
       const BlockScale<NV> sc(__float_as_uint(top), p.xq);
-      const uint32_t w = quantize8<NV>(sc, v);
       // 128-byte rows, 16-byte pieces swizzled by the row
-      *reinterpret_cast<uint32_t *>(codes + (size_t)s * p.NT * 128 + t * 128 + (((lane >> 2) ^ (t & 7)) << 4) + (lane & 3) * 4) = w;
+      *reinterpret_cast<uint32_t *>(codes + (s * p.NT + t) * 128 + (((lane >> 2) ^ (t & 7)) << 4) + (lane & 3) * 4) =
+          quantize8<NV>(sc, v);
       if (lane % LB == 0)
         scales[(s * AT + lane / (4 * LB)) * 512 + (t & 31) * 16 + (t >> 5) * 4 + lane / LB % 4] =
             k_begin + s * 256 + lane * 8 < p.a.K ? (uint8_t)sc.byte : 0;
+    };
+    if (i0 + (U - 1) * W < n) {  // without branches between them the pieces overlap
+#pragma unroll
+      for (int u = 0; u < U; ++u) piece(u);
+    } else {
+#pragma unroll
+      for (int u = 0; u < U - 1; ++u)
+        if (i0 + u * W < n) piece(u);
     }
+  }
+}
+
+// The results of a tile.  Warps 0 .. 3 and 4 .. 7 take alternate groups of 16
+// tokens; a thread has one weight row.  The slices' partial sums go to the CTA
+// that adds them as [source][four tokens][gate, up][row][token], 16 bytes a
+// thread.  OT: result type, -1 the 4-bit result.
+template <bool NV, bool GLU, int OT>
+T0B_DEV void split_results(const SplitArgs &p, uint8_t *slots, uint32_t tmem, int rank, int n0, int m0, int toks, bool have) {
+  constexpr int H = GLU ? 2 : 1, TY = OT < 0 ? TY_F32 : OT;
+  const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const int NT = p.NT, CS = p.CS;
+  const int half = warp >> 2, row = 32 * (warp & 3) + lane, n = n0 + row;
+  const int sh4 = ((NT + CS - 1) / CS + 3) / 4;  // groups of four tokens whose slices a CTA adds
+  const uint32_t trow = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
+  const float alpha = p.a.alpha;
+  float b0 = 0.0f, b1 = 0.0f;
+  if (p.a.bias && n < p.a.n) {
+    b0 = p.a.bias[n];
+    if (GLU) b1 = p.a.bias[p.a.n + n];
+  }
+  typename Plain<TY>::T *y = reinterpret_cast<typename Plain<TY>::T *>(p.a.y) + m0 * p.a.ld + n;
+  const bool in = n < p.a.n;
+  auto finish4 = [&](int t0, const float *g, const float *u) {  // tokens t0 .. t0 + 3 of the tile
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float v = fmaf(g[j], alpha, b0);
+      if constexpr (GLU) v = silu_mul(v, fmaf(u[j], alpha, b1));
+      if constexpr (OT >= 0) {
+        if (in && t0 + j < toks) y[(t0 + j) * p.a.ld] = Plain<TY>::put(v);
+      } else {
+        if (t0 + j < toks) quantize_lanes<NV>(p.a.q, m0 + t0 + j, n0 + 32 * (warp & 3), in ? v : 0.0f);
+      }
+    }
+  };
+  for (int t0 = 16 * half; t0 < toks && have; t0 += 32) {
+    uint32_t g[16], u[16];
+    tmem_ld16(trow + t0, g);
+    if (GLU) tmem_ld16(trow + NT + t0, u);
+    tmem_ld_wait16(g);
+    if (GLU) tmem_ld_wait16(u);
+    const float *gf = reinterpret_cast<const float *>(g), *uf = reinterpret_cast<const float *>(u);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const int c4 = t0 / 4 + c;
+      if (4 * c4 >= toks) break;
+      if (CS == 1) {
+        finish4(4 * c4, gf + 4 * c, uf + 4 * c);
+      } else {
+        const int owner = c4 / sh4;
+        const uint32_t at = mapa_shared(smem_u32(slots) + (((rank * sh4 + c4 - owner * sh4) * H) * 128 + row) * 16, owner);
+        st_cluster_f32x4(at, gf + 4 * c);
+        if (GLU) st_cluster_f32x4(at + 2048, uf + 4 * c);
+      }
+    }
+  }
+  tc_fence_before();
+  __syncwarp();
+  if (CS > 1) {
+    cluster_sync_all();
+    const float4 *slot = reinterpret_cast<const float4 *>(slots) + row;
+    for (int c4 = half; c4 < sh4 && have; c4 += 2) {
+      const int t0 = 4 * (rank * sh4 + c4);
+      if (t0 >= toks) break;
+      float4 g[2] = {};
+#pragma unroll
+      for (int c = 0; c < SPLIT_MAX_CLUSTER; ++c) {
+        if (c >= CS) break;
+        const float4 *v = slot + (c * sh4 + c4) * H * 128;
+        add4(g[0], v[0]);
+        if (GLU) add4(g[1], v[128]);
+      }
+      finish4(t0, &g[0].x, &g[1].x);
+    }
+  } else {
+    __syncthreads();
+  }
+  if (OT < 0 && m0 + NT >= p.a.M && rank == 0) {
+    // zero scales of the last row group's rows behind the last token
+    const int m = p.a.M + (int)threadIdx.x % 128;
+    constexpr int TILES = NV ? 2 : 1;  // scale tiles of 128 columns
+    const int t = n0 / 128 * TILES + (int)threadIdx.x / 128, kt = (p.a.q.k + (NV ? 63 : 127)) / (NV ? 64 : 128);
+    if (m < (p.a.M + 127) / 128 * 128 && (int)threadIdx.x / 128 < TILES && t < kt)
+      *reinterpret_cast<uint32_t *>(p.a.q.scales + scale_at(m, 4 * t, kt)) = 0;
   }
 }
 
@@ -1133,83 +1228,18 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 1)
   __syncwarp();
   if (CS > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
 
-  // ------------------------------------------------------------ results
-  // Warps 0 .. 3 and 4 .. 7 take alternate groups of eight tokens; a thread has
-  // one weight row.  The slices' partial sums go to the CTA that adds them as
-  // [source][four tokens][gate, up][row][token], 16 bytes a thread.
-  const int half = warp >> 2, row = 32 * (warp & 3) + lane, n = n0 + row;
-  const int sh4 = ((NT + CS - 1) / CS + 3) / 4;  // groups of four tokens whose slices a CTA adds
-  const uint32_t trow = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
-  float b0 = 0.0f, b1 = 0.0f;
-  if (p.a.bias && n < p.a.n) {
-    b0 = p.a.bias[n];
-    if (GLU) b1 = p.a.bias[p.a.n + n];
-  }
-  auto finish = [&](int t, float g, float u) {  // token t of the tile
-    const int m = m0 + t;
-    float v = fmaf(g, p.a.alpha, b0);
-    if constexpr (GLU) v = silu_mul(v, fmaf(u, p.a.alpha, b1));
-    if (p.out_type >= 0) {
-      if (n < p.a.n) store_elem(p.a.y, p.out_type, m * p.a.ld + n, v);
-    } else if constexpr (GLU) {
-      quantize_lanes<NV>(p.a.q, m, n0 + 32 * (warp & 3), n < p.a.n ? v : 0.0f);
-    }
-  };
   bool have = mbar_wait(acc_full, 0, p.a.err, T0B_DEVERR_WAIT_ACC, abort_flag) && !*abort_flag;
   have = __all_sync(0xFFFFFFFFu, have);
   tc_fence_after();
-  for (int t0 = 8 * half; t0 < toks && have; t0 += 16) {
-    float g[8], u[8];
-    tmem_ld8(trow + t0, g);
-    if (GLU) tmem_ld8(trow + NT + t0, u);
-    if (CS == 1) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (t0 + j < toks) finish(t0 + j, g[j], GLU ? u[j] : 0.0f);
-    } else {
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const int c4 = t0 / 4 + c, owner = c4 / sh4;
-        if (owner >= CS) break;
-        const uint32_t at =
-            mapa_shared(smem_u32(smem + p.off_slot) + (((rank * sh4 + c4 - owner * sh4) * H) * 128 + row) * 16, owner);
-        st_cluster_f32x4(at, g + 4 * c);
-        if (GLU) st_cluster_f32x4(at + 2048, u + 4 * c);
-      }
-    }
-  }
-  tc_fence_before();
-  __syncwarp();
-  if (CS > 1) {
-    cluster_sync_all();
-    const float4 *slot = reinterpret_cast<const float4 *>(smem + p.off_slot) + row;
-    for (int c4 = half; c4 < sh4 && have; c4 += 2) {
-      const int t0 = 4 * (rank * sh4 + c4);
-      if (t0 >= toks) break;
-      float4 g = make_float4(0.f, 0.f, 0.f, 0.f), u = g;
-#pragma unroll
-      for (int c = 0; c < SPLIT_MAX_CLUSTER; ++c) {
-        if (c >= CS) break;
-        const float4 *v = slot + (c * sh4 + c4) * H * 128;
-        add4(g, v[0]);
-        if (GLU) add4(u, v[128]);
-      }
-      finish(t0, g.x, u.x);
-      if (t0 + 1 < toks) finish(t0 + 1, g.y, u.y);
-      if (t0 + 2 < toks) finish(t0 + 2, g.z, u.z);
-      if (t0 + 3 < toks) finish(t0 + 3, g.w, u.w);
-    }
-  } else {
-    __syncthreads();
-  }
-  if (GLU && p.out_type < 0 && m0 + NT >= p.a.M && rank == 0) {
-    // zero scales of the last row group's rows behind the last token
-    const int m = p.a.M + (int)threadIdx.x % 128;
-    constexpr int TILES = NV ? 2 : 1;  // scale tiles of 128 columns
-    const int t = n0 / 128 * TILES + (int)threadIdx.x / 128, kt = (p.a.q.k + (NV ? 63 : 127)) / (NV ? 64 : 128);
-    if (m < (p.a.M + 127) / 128 * 128 && (int)threadIdx.x / 128 < TILES && t < kt)
-      *reinterpret_cast<uint32_t *>(p.a.q.scales + scale_at(m, 4 * t, kt)) = 0;
-  }
+  uint8_t *slots = smem + p.off_slot;
+  if (GLU && p.out_type < 0)
+    split_results<NV, GLU, -1>(p, slots, tmem, rank, n0, m0, toks, have);
+  else if (p.out_type == TY_F32)
+    split_results<NV, GLU, TY_F32>(p, slots, tmem, rank, n0, m0, toks, have);
+  else if (p.out_type == TY_F16)
+    split_results<NV, GLU, TY_F16>(p, slots, tmem, rank, n0, m0, toks, have);
+  else
+    split_results<NV, GLU, TY_BF16>(p, slots, tmem, rank, n0, m0, toks, have);
   __syncwarp();
   if (warp == 1) {
     tc_fence_after();
@@ -1285,19 +1315,44 @@ int sm_count() {
 struct SplitPlan {
   int NT, CS, SL, rt;
   int64_t ctas;
+  double us;  // estimate
 };
-SplitPlan split_plan(bool glu, int M, int n, int K, int sms) {
+// Tiles of 64 or 128 tokens where one does not hold them all (the scale columns
+// of a tile's first token have to be even: multiples of 64 tokens).
+SplitPlan split_plan(bool glu, int M, int n, int K, int most, int sms) {
   SplitPlan q;
-  const int most = glu ? 64 : 128;  // tokens of a tile; several tiles start at whole scale columns
   q.NT = M <= most ? (M + 7) / 8 * 8 : most;
   q.rt = (n + 127) / 128;
   const int64_t tiles = (int64_t)q.rt * ((M + q.NT - 1) / q.NT);
   const int S = (K + 255) / 256;
+  // clusters have to fit the GPCs: of 8 CTAs not more than two thirds of the
+  // SMs can be used at once
   int cs = 1;
-  while (cs < SPLIT_MAX_CLUSTER && tiles * cs * 2 <= sms && S >= cs * 2) cs *= 2;
+  while (cs < SPLIT_MAX_CLUSTER && tiles * cs * 2 <= (cs == 4 ? sms * 2 / 3 : sms * 7 / 8) && S >= cs * 2) cs *= 2;
   q.SL = (S + cs - 1) / cs;
   q.CS = (S + q.SL - 1) / q.SL;
   q.ctas = tiles * q.CS;
+  // microseconds, fitted to the measured times (within 15 % where either
+  // kernel is chosen): 512 x 512 3.3 (16 tokens), 4.6 (64); 8192 x 8192 9.8
+  // (16), 13.8 (128), 18.7 (256)
+  const double waves = (double)((q.ctas + sms - 1) / sms);
+  q.us = 2.6 + waves * ((glu ? 0.045 : 0.030) * q.NT + (glu ? 0.7 : 0.4) * q.SL);
+  return q;
+}
+// The same for the pair kernel: 256 tokens 512 x 512 4.8, 1024 x 4096 8.9,
+// 8192 x 8192 14.1; gated 512 x 512 5.5, 4096 x 4096 10.1.
+double pair_us(bool glu, int M, int n, int K, int sms) {
+  const int64_t tiles = (int64_t)((M + 255) / 256) * (glu ? (n + 127) / 128 : (n + 255) / 256);
+  return 3.9 + (double)((tiles + sms / 2 - 1) / (sms / 2)) * ((glu ? 1.1 : 0.5) + 0.31 * ((K + 255) / 256));
+}
+// The split kernel's plan if it is the faster one (CS 0: the pair kernel is).
+SplitPlan choose(bool glu, int M, int n, int K, int sms) {
+  SplitPlan q = split_plan(glu, M, n, K, 64, sms);
+  if (!glu && M > 64) {
+    const SplitPlan r = split_plan(glu, M, n, K, 128, sms);
+    if (r.us < q.us) q = r;
+  }
+  if (pair_us(glu, M, n, K, sms) <= q.us) q.CS = 0;
   return q;
 }
 
@@ -1470,15 +1525,12 @@ Fp4Args product_args(const Fp4Mat &w, const Fp4Mat &x, const Fp4Out &out, int *e
   return p;
 }
 
-// Tokens up to which a CTA of the split kernel quantises plain activations
-// itself.
-constexpr int FUSED_MAX_TOKENS = 32;
-
-bool use_split(const Fp4Args &a, bool glu, const SplitPlan &q, int sms) {
-  const int64_t pair_tiles = (int64_t)((a.M + 255) / 256) * (glu ? (a.n + 127) / 128 : (a.n + 255) / 256);
-  (void)q;
-  return a.M <= 256 || 4 * pair_tiles <= sms;
-}
+// Values of the activations up to which a CTA of the split kernel quantises
+// its slice itself (a piece of 256 takes a warp 0.26 us).  4096 x 4096, 16
+// tokens (at the limit): 7.3 us in a graph and 7.9 us a call, with a quantise
+// launch 6.6 and 8.7; 32 tokens: 9.7 and 9.9, with a launch 7.0 and 8.8; 1
+// token: 5.4 and 6.5, with a launch 6.1 and 9.2.
+constexpr int FUSED_MAX_VALUES = 16384;
 
 template <bool FUSED>
 cudaError_t split_dispatch(const Fp4Mat &w, const Fp4Mat &xm, const void *x, int x_type, int64_t ldx, const Fp4Out &out,
@@ -1495,19 +1547,19 @@ cudaError_t split_dispatch(const Fp4Mat &w, const Fp4Mat &xm, const void *x, int
 
 cudaError_t t0b_launch_fp4_gemm(const Fp4Mat &w, const Fp4Mat &x, const Fp4Out &out, bool after_own, int *err, cudaStream_t st) {
   const Fp4Args a = product_args(w, x, out, err);
-  const int sms = sm_count();
-  const SplitPlan q = split_plan(out.glu, a.M, a.n, a.K, sms);
-  if (use_split(a, out.glu, q, sms)) return split_dispatch<false>(w, x, nullptr, -1, 0, out, a, q, after_own, st);
+  const SplitPlan q = choose(out.glu, a.M, a.n, a.K, sm_count());
+  if (q.CS) return split_dispatch<false>(w, x, nullptr, -1, 0, out, a, q, after_own, st);
   return w.blk == 16 ? gemm_fmt<true>(w, x, out, a, st) : gemm_fmt<false>(w, x, out, a, st);
 }
 
 cudaError_t t0b_launch_fp4_linear(const Fp4Mat &w, int x_type, const void *x, int64_t ldx, const Fp4Mat &xq, const Fp4Out &out,
                                   int *err, cudaStream_t st) {
-  if (xq.rows <= FUSED_MAX_TOKENS) {
+  if (xq.rows <= 64) {
     const Fp4Args a = product_args(w, xq, out, err);
-    const SplitPlan q = split_plan(out.glu, a.M, a.n, a.K, sm_count());
+    const SplitPlan q = choose(out.glu, a.M, a.n, a.K, sm_count());
     // its share of the activations stays in shared memory
-    if (q.SL <= 8) return split_dispatch<true>(w, xq, x, x_type, ldx, out, a, q, false, st);
+    if (q.CS && q.SL <= 8 && q.SL * 256 * a.M <= FUSED_MAX_VALUES)
+      return split_dispatch<true>(w, xq, x, x_type, ldx, out, a, q, false, st);
   }
   const cudaError_t e = t0b_launch_fp4_quantize(x_type, x, ldx, xq, st);
   return e != cudaSuccess ? e : t0b_launch_fp4_gemm(w, xq, out, true, err, st);
