@@ -447,7 +447,7 @@ T0B_DEV void umma_fp4_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, u
 // One lane of a converged warp, known to the compiler as such: what it issues
 // keeps its operands in uniform registers.  (Chosen by `lane == 0`, the MMA
 // warp issued an 8192 x 8192 x 8192 product's instructions in 360 us instead
-// of 193.)
+// of 193; loops and waits stay with the whole warp.)
 T0B_DEV bool elect_one() {
   uint32_t ok;
   asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xFFFFFFFF;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(ok));
@@ -675,40 +675,51 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
         }
       }
     }
-  } else if (warp == 1 && rank == 0 && elect_one()) {
+  } else if (warp == 1 && rank == 0) {
     // ------------------------------------------------------------ MMA (CTA 0)
     constexpr uint32_t idesc = idesc_fp4<NV>(256, 256);
-    uint32_t g = 0, it = 0;
     const int steps = (p.K + 63) / 64;
-    for (int tile = pair; tile < p.n_tiles && !*abort_flag; tile += npairs, ++it) {
-      if (it >= 1 && !mbar_wait(acc_empty, (it - 1) & 1, p.err, T0B_DEVERR_WAIT_ACC, abort_flag)) break;
+    const uint64_t da = sw128_desc(base + C::OFF_A), db = sw128_desc(base + C::OFF_B);
+    const uint64_t dsa = scale_desc(base + C::OFF_SA), dsb = scale_desc(base + C::OFF_SB);
+    uint32_t sl = 0, phase = 0, it = 0;
+    bool ok = true;
+    for (int tile = pair; tile < p.n_tiles && ok; tile += npairs, ++it) {
+      if (it >= 1) ok = mbar_wait(acc_empty, (it - 1) & 1, p.err, T0B_DEVERR_WAIT_ACC, abort_flag);
+      ok = __all_sync(0xFFFFFFFFu, ok);
+      if (!ok) break;
       tc_fence_after();
-      for (int s = 0; s < S; ++s, ++g) {
-        const uint32_t sl = g % NS;
-        if (!mbar_wait(&full[sl], (g / NS) & 1, p.err, T0B_DEVERR_WAIT_X, abort_flag)) break;
-        if (ROT && !mbar_wait(&rot_full[sl], (g / NS) & 1, p.err, T0B_DEVERR_WAIT_DEQ, abort_flag)) break;
+      for (int s = 0; s < S; ++s) {
+        ok = mbar_wait(&full[sl], phase, p.err, T0B_DEVERR_WAIT_X, abort_flag) &&
+             (!ROT || mbar_wait(&rot_full[sl], phase, p.err, T0B_DEVERR_WAIT_DEQ, abort_flag));
+        ok = __all_sync(0xFFFFFFFFu, ok);
+        if (!ok) break;
         tc_fence_after();
-        const uint32_t st = base + sl * C::STAGE, sf = tmem + 256 + sl * C::SFC;
+        const uint64_t at = sl * (C::STAGE >> 4);
+        const uint32_t sf = tmem + 256 + sl * C::SFC;
+        const int n = steps - 4 * s;
+        if (elect_one()) {
 #pragma unroll
-        for (int a = 0; a < AT; ++a) {
-          scale_cp_pair(sf + 4 * a, scale_desc(st + C::OFF_SA + 512 * a));
-          scale_cp_pair(sf + 4 * AT + 8 * a, scale_desc(st + C::OFF_SB + 512 * a));
-          scale_cp_pair(sf + 4 * AT + 8 * a + 4, scale_desc(st + C::OFF_SB + C::SC + 512 * a));
-        }
+          for (int a = 0; a < AT; ++a) {
+            scale_cp_pair(sf + 4 * a, dsa + at + 32 * a);
+            scale_cp_pair(sf + 4 * AT + 8 * a, dsb + at + 32 * a);
+            scale_cp_pair(sf + 4 * AT + 8 * a + 4, dsb + at + (C::SC >> 4) + 32 * a);
+          }
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk) {
-          if (4 * s + kk >= steps) break;
-          const int a = NV ? kk : kk / 2;
-          umma_fp4_pair<NV>(tmem, sw128_desc(st + C::OFF_A + 32 * kk), sw128_desc(st + C::OFF_B + 32 * kk),
-                            idesc | (NV ? 0u : idesc_scale_id(kk % 2 * 2)), sf + 4 * a, sf + 4 * AT + 8 * a,
-                            s > 0 || kk > 0);
+          for (int kk = 0; kk < 4; ++kk)
+            if (kk < n) {
+              const int a = NV ? kk : kk / 2;
+              umma_fp4_pair<NV>(tmem, da + at + 2 * kk, db + at + 2 * kk, idesc | (NV ? 0u : idesc_scale_id(kk % 2 * 2)),
+                                sf + 4 * a, sf + 4 * AT + 8 * a, s > 0 || kk > 0);
+            }
+          umma_commit_pair_both(&empty[sl]);
+          if (s == S - 1) umma_commit_pair_both(acc_full);
         }
-        umma_commit_pair_both(&empty[sl]);
+        __syncwarp();
+        if (++sl == NS) sl = 0, phase ^= 1;
       }
-      if (*abort_flag) break;
-      umma_commit_pair_both(acc_full);
     }
-    umma_commit_pair(smem_u32(mma_done));
+    if (elect_one()) umma_commit_pair(smem_u32(mma_done));
+    __syncwarp();
     mbar_wait(mma_done, 0, p.err, T0B_DEVERR_WAIT_ACC, nullptr);
   } else if (ROT && warp == 2) {
     // ------------------------------------------------------------ up rows' scales (both CTAs)
@@ -1105,6 +1116,14 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 1)
     *abort_flag = 0;
     fence_barrier_init();
     fence_proxy_async_smem();
+  }
+  if (warp == 2 && lane == 0) {
+    prefetch_tmap(&tm_w);
+    prefetch_tmap(&tm_ws);
+    if (!FUSED) {
+      prefetch_tmap(&tm_x);
+      prefetch_tmap(&tm_xs);
+    }
   }
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(p.tmem_cols)
