@@ -551,7 +551,7 @@ T0B_DEV void store_rows(const Fp4Args &p, const void *tm_y, uint8_t *stg, int ro
     fence_proxy_async_smem();
     __syncwarp();
     if (lane == 0) {
-      if (row0 < p.M && c0 < p.n) tma_store_2d(tm_y, stg, c0, row0);
+      if (row0 < p.M && c0 < p.n && T0B_CHECK_TMA(c0, (int)sizeof(T), row0, p.err)) tma_store_2d(tm_y, stg, c0, row0);
       bulk_commit();
     }
   } else {
@@ -660,6 +660,7 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
         uint8_t *st = smem + sl * C::STAGE;
         if (rank == 0) mbar_arrive_expect_tx(&full[sl], 4 * C::CODES + (ROT ? 4 : 6) * C::SC);
         const uint32_t fb = lead(&full[sl]);
+        if (!T0B_CHECK_TMA(s * 128, 1, m0, p.err) || !T0B_CHECK(w_row(nt, 1) >= 0 && s * AT < p.kt, p.err)) continue;
         // (byte, row) of the codes, (tile, row group) of the scales; what lies
         // behind the matrix arrives as zeros
         tma_load_2d_pair(st + C::OFF_A, &tm_x, fb, s * 128, m0);
@@ -1139,6 +1140,7 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 1)
   auto load_w = [&](int i) {  // stage i of the slice
     const int sl = i % NS, s = s0 + i;
     uint8_t *st = smem + sl * p.stage;
+    if (!T0B_CHECK_TMA(s * 128, 1, n0, p.a.err) || !T0B_CHECK(s * AT < p.a.kt && sl < SPLIT_MAX_NS, p.a.err)) return;
     const bool rot = GLU && p.rot;
     mbar_arrive_expect_tx(&full[sl], H * 16384u + (GLU && !rot ? 2 : 1) * SC + (FUSED ? 0u : (uint32_t)NT * 128u + SC));
     tma_load_2d(st, &tm_w, &full[sl], s * 128, n0);
@@ -1158,6 +1160,7 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 1)
   auto load_x = [&](int i) {
     const int sl = i % NS, s = s0 + i;
     uint8_t *st = smem + sl * p.stage;
+    if (!T0B_CHECK_TMA(s * 128, 1, m0, p.a.err)) return;
     tma_load_2d(st + OFF_X, &tm_x, &full[sl], s * 128, m0);
     tma_load_3d(st + OFF_XS, &tm_xs, &full[sl], 0, s * AT, m0 >> 7);
   };

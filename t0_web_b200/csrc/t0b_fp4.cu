@@ -104,6 +104,17 @@ t0b_status cuda_status(const char *fn, cudaError_t e) {
   return fail(T0B_ERR_CUDA, fn, cudaGetErrorString(e));
 }
 
+// A C entry's body: no C++ exception leaves it (the host-side caches and the
+// error message allocate).
+template <class F>
+t0b_status guarded(F body) {
+  try {
+    return body();
+  } catch (...) {
+    return T0B_ERR_OOM;
+  }
+}
+
 #define TRY(expr)                        \
   do {                                   \
     const t0b_status s_ = (expr);        \
@@ -125,129 +136,143 @@ extern "C" size_t t0b_fp4_scale_bytes(int format, int rows, int k) {
 
 extern "C" t0b_status t0b_fp4_quantize(t0b_engine *e, int x_type, const void *x_dev, int64_t ldx, const t0b_fp4 *out,
                                        void *stream) {
-  const char *fn = "t0b_fp4_quantize";
-  if (!e) return fail(T0B_ERR_INVALID, fn, "engine is NULL");
-  Fp4Mat q;
-  TRY(check_mat(fn, "out", out, true, &q));
-  TRY(check_plain(fn, "x", x_type, x_dev, ldx, q.rows, q.k));
-  DeviceScope dev(t0b_engine_device(e));
-  TRY(cuda_status(fn, dev.status));
-  return cuda_status(fn, t0b_launch_fp4_quantize(x_type, x_dev, ldx, q, (cudaStream_t)stream));
+  return guarded([&]() -> t0b_status {
+    const char *fn = "t0b_fp4_quantize";
+    if (!e) return fail(T0B_ERR_INVALID, fn, "engine is NULL");
+    Fp4Mat q;
+    TRY(check_mat(fn, "out", out, true, &q));
+    TRY(check_plain(fn, "x", x_type, x_dev, ldx, q.rows, q.k));
+    DeviceScope dev(t0b_engine_device(e));
+    TRY(cuda_status(fn, dev.status));
+    return cuda_status(fn, t0b_launch_fp4_quantize(x_type, x_dev, ldx, q, (cudaStream_t)stream));
+  });
 }
 
 extern "C" t0b_status t0b_fp4_dequantize(t0b_engine *e, const t0b_fp4 *in, int y_type, void *y_dev, int64_t ldy,
                                          void *stream) {
-  const char *fn = "t0b_fp4_dequantize";
-  if (!e) return fail(T0B_ERR_INVALID, fn, "engine is NULL");
-  Fp4Mat q;
-  TRY(check_mat(fn, "in", in, false, &q));
-  TRY(check_plain(fn, "y", y_type, y_dev, ldy, q.rows, q.k));
-  DeviceScope dev(t0b_engine_device(e));
-  TRY(cuda_status(fn, dev.status));
-  return cuda_status(fn, t0b_launch_fp4_dequantize(q, y_type, y_dev, ldy, (cudaStream_t)stream));
+  return guarded([&]() -> t0b_status {
+    const char *fn = "t0b_fp4_dequantize";
+    if (!e) return fail(T0B_ERR_INVALID, fn, "engine is NULL");
+    Fp4Mat q;
+    TRY(check_mat(fn, "in", in, false, &q));
+    TRY(check_plain(fn, "y", y_type, y_dev, ldy, q.rows, q.k));
+    DeviceScope dev(t0b_engine_device(e));
+    TRY(cuda_status(fn, dev.status));
+    return cuda_status(fn, t0b_launch_fp4_dequantize(q, y_type, y_dev, ldy, (cudaStream_t)stream));
+  });
 }
 
 extern "C" t0b_status t0b_fp4_gemm(t0b_engine *e, const t0b_fp4 *w, const t0b_fp4 *x, const float *bias_dev, int y_type,
                                    void *y_dev, int64_t ldy, void *stream) {
-  const char *fn = "t0b_fp4_gemm";
-  if (!e) return fail(T0B_ERR_INVALID, fn, "engine is NULL");
-  Fp4Mat wm, xm;
-  TRY(check_mat(fn, "w", w, false, &wm));
-  TRY(check_mat(fn, "x", x, false, &xm));
-  TRY(check_product(fn, wm, xm));
-  TRY(check_bias(fn, bias_dev));
-  TRY(check_plain(fn, "y", y_type, y_dev, ldy, xm.rows, wm.rows));
-  DeviceScope dev(t0b_engine_device(e));
-  TRY(cuda_status(fn, dev.status));
-  const Fp4Out out{y_type, y_dev, ldy, bias_dev, false, false, {}};
-  return cuda_status(fn, t0b_launch_fp4_gemm(wm, xm, out, false, t0b_engine_fp4_err(e), (cudaStream_t)stream));
+  return guarded([&]() -> t0b_status {
+    const char *fn = "t0b_fp4_gemm";
+    if (!e) return fail(T0B_ERR_INVALID, fn, "engine is NULL");
+    Fp4Mat wm, xm;
+    TRY(check_mat(fn, "w", w, false, &wm));
+    TRY(check_mat(fn, "x", x, false, &xm));
+    TRY(check_product(fn, wm, xm));
+    TRY(check_bias(fn, bias_dev));
+    TRY(check_plain(fn, "y", y_type, y_dev, ldy, xm.rows, wm.rows));
+    DeviceScope dev(t0b_engine_device(e));
+    TRY(cuda_status(fn, dev.status));
+    const Fp4Out out{y_type, y_dev, ldy, bias_dev, false, false, {}};
+    return cuda_status(fn, t0b_launch_fp4_gemm(wm, xm, out, false, t0b_engine_fp4_err(e), (cudaStream_t)stream));
+  });
 }
 
 extern "C" t0b_status t0b_fp4_glu(t0b_engine *e, const t0b_fp4 *w, const t0b_fp4 *x, const float *bias_dev, int z_type,
                                   void *z_dev, int64_t ldz, const t0b_fp4 *zq, void *stream) {
-  const char *fn = "t0b_fp4_glu";
-  if (!e) return fail(T0B_ERR_INVALID, fn, "engine is NULL");
-  if ((z_dev != nullptr) == (zq != nullptr)) return fail(T0B_ERR_INVALID, fn, "needs either z_dev or zq");
-  Fp4Mat wm, xm;
-  TRY(check_mat(fn, "w", w, false, &wm));
-  TRY(check_mat(fn, "x", x, false, &xm));
-  TRY(check_product(fn, wm, xm));
-  TRY(check_bias(fn, bias_dev));
-  if (wm.rows % 2) return fail(T0B_ERR_INVALID, fn, "w needs gate and up rows in equal number");
-  const int F = wm.rows / 2;
-  Fp4Out out{z_type, z_dev, ldz, bias_dev, true, zq != nullptr, {}};
-  if (zq) {
-    TRY(check_mat(fn, "zq", zq, true, &out.q));
-    if (out.q.blk != wm.blk || out.q.rows != xm.rows || out.q.k != F)
-      return fail(T0B_ERR_INVALID, fn, "zq must have w's format and shape [x->rows, w->rows / 2]");
-  } else {
-    TRY(check_plain(fn, "z", z_type, z_dev, ldz, xm.rows, F));
-  }
-  DeviceScope dev(t0b_engine_device(e));
-  TRY(cuda_status(fn, dev.status));
-  return cuda_status(fn, t0b_launch_fp4_gemm(wm, xm, out, false, t0b_engine_fp4_err(e), (cudaStream_t)stream));
+  return guarded([&]() -> t0b_status {
+    const char *fn = "t0b_fp4_glu";
+    if (!e) return fail(T0B_ERR_INVALID, fn, "engine is NULL");
+    if ((z_dev != nullptr) == (zq != nullptr)) return fail(T0B_ERR_INVALID, fn, "needs either z_dev or zq");
+    Fp4Mat wm, xm;
+    TRY(check_mat(fn, "w", w, false, &wm));
+    TRY(check_mat(fn, "x", x, false, &xm));
+    TRY(check_product(fn, wm, xm));
+    TRY(check_bias(fn, bias_dev));
+    if (wm.rows % 2) return fail(T0B_ERR_INVALID, fn, "w needs gate and up rows in equal number");
+    const int F = wm.rows / 2;
+    Fp4Out out{z_type, z_dev, ldz, bias_dev, true, zq != nullptr, {}};
+    if (zq) {
+      TRY(check_mat(fn, "zq", zq, true, &out.q));
+      if (out.q.blk != wm.blk || out.q.rows != xm.rows || out.q.k != F)
+        return fail(T0B_ERR_INVALID, fn, "zq must have w's format and shape [x->rows, w->rows / 2]");
+    } else {
+      TRY(check_plain(fn, "z", z_type, z_dev, ldz, xm.rows, F));
+    }
+    DeviceScope dev(t0b_engine_device(e));
+    TRY(cuda_status(fn, dev.status));
+    return cuda_status(fn, t0b_launch_fp4_gemm(wm, xm, out, false, t0b_engine_fp4_err(e), (cudaStream_t)stream));
+  });
 }
 
 extern "C" t0b_status t0b_fp4_linear(t0b_engine *e, const t0b_fp4 *w, int x_type, const void *x_dev, int64_t ldx,
                                      const t0b_fp4 *xq, const float *bias_dev, int y_type, void *y_dev, int64_t ldy,
                                      void *stream) {
-  const char *fn = "t0b_fp4_linear";
-  if (!e) return fail(T0B_ERR_INVALID, fn, "engine is NULL");
-  Fp4Mat wm, xm;
-  TRY(check_mat(fn, "w", w, false, &wm));
-  TRY(check_mat(fn, "xq", xq, true, &xm));
-  TRY(check_product(fn, wm, xm));
-  TRY(check_bias(fn, bias_dev));
-  TRY(check_plain(fn, "x", x_type, x_dev, ldx, xm.rows, xm.k));
-  TRY(check_plain(fn, "y", y_type, y_dev, ldy, xm.rows, wm.rows));
-  DeviceScope dev(t0b_engine_device(e));
-  TRY(cuda_status(fn, dev.status));
-  const Fp4Out out{y_type, y_dev, ldy, bias_dev, false, false, {}};
-  return cuda_status(fn, t0b_launch_fp4_linear(wm, x_type, x_dev, ldx, xm, out, t0b_engine_fp4_err(e), (cudaStream_t)stream));
+  return guarded([&]() -> t0b_status {
+    const char *fn = "t0b_fp4_linear";
+    if (!e) return fail(T0B_ERR_INVALID, fn, "engine is NULL");
+    Fp4Mat wm, xm;
+    TRY(check_mat(fn, "w", w, false, &wm));
+    TRY(check_mat(fn, "xq", xq, true, &xm));
+    TRY(check_product(fn, wm, xm));
+    TRY(check_bias(fn, bias_dev));
+    TRY(check_plain(fn, "x", x_type, x_dev, ldx, xm.rows, xm.k));
+    TRY(check_plain(fn, "y", y_type, y_dev, ldy, xm.rows, wm.rows));
+    DeviceScope dev(t0b_engine_device(e));
+    TRY(cuda_status(fn, dev.status));
+    const Fp4Out out{y_type, y_dev, ldy, bias_dev, false, false, {}};
+    return cuda_status(fn, t0b_launch_fp4_linear(wm, x_type, x_dev, ldx, xm, out, t0b_engine_fp4_err(e), (cudaStream_t)stream));
+  });
 }
 
 extern "C" t0b_status t0b_fp4_mlp(t0b_engine *e, const t0b_fp4 *w0, const t0b_fp4 *w2, int x_type, const void *x_dev,
                                   int64_t ldx, const t0b_fp4 *xq, const t0b_fp4 *zq, const float *b0_dev,
                                   const float *b2_dev, int y_type, void *y_dev, int64_t ldy, void *stream) {
-  const char *fn = "t0b_fp4_mlp";
-  if (!e) return fail(T0B_ERR_INVALID, fn, "engine is NULL");
-  Fp4Mat w0m, w2m, xm, zm;
-  TRY(check_mat(fn, "w0", w0, false, &w0m));
-  TRY(check_mat(fn, "w2", w2, false, &w2m));
-  TRY(check_mat(fn, "xq", xq, true, &xm));
-  TRY(check_mat(fn, "zq", zq, true, &zm));
-  TRY(check_product(fn, w0m, xm));
-  TRY(check_product(fn, w2m, zm));
-  TRY(check_bias(fn, b0_dev));
-  TRY(check_bias(fn, b2_dev));
-  if (w0m.rows % 2) return fail(T0B_ERR_INVALID, fn, "w0 needs gate and up rows in equal number");
-  if (zm.rows != xm.rows || zm.k != w0m.rows / 2 || zm.blk != w0m.blk)
-    return fail(T0B_ERR_INVALID, fn, "zq must have w0's format and shape [xq->rows, w0->rows / 2]");
-  TRY(check_plain(fn, "x", x_type, x_dev, ldx, xm.rows, xm.k));
-  TRY(check_plain(fn, "y", y_type, y_dev, ldy, xm.rows, w2m.rows));
-  DeviceScope dev(t0b_engine_device(e));
-  TRY(cuda_status(fn, dev.status));
-  const cudaStream_t st = (cudaStream_t)stream;
-  int *err = t0b_engine_fp4_err(e);
-  const Fp4Out hid{0, nullptr, 0, b0_dev, true, true, zm};
-  TRY(cuda_status(fn, t0b_launch_fp4_linear(w0m, x_type, x_dev, ldx, xm, hid, err, st)));
-  const Fp4Out out{y_type, y_dev, ldy, b2_dev, false, false, {}};
-  return cuda_status(fn, t0b_launch_fp4_gemm(w2m, zm, out, true, err, st));
+  return guarded([&]() -> t0b_status {
+    const char *fn = "t0b_fp4_mlp";
+    if (!e) return fail(T0B_ERR_INVALID, fn, "engine is NULL");
+    Fp4Mat w0m, w2m, xm, zm;
+    TRY(check_mat(fn, "w0", w0, false, &w0m));
+    TRY(check_mat(fn, "w2", w2, false, &w2m));
+    TRY(check_mat(fn, "xq", xq, true, &xm));
+    TRY(check_mat(fn, "zq", zq, true, &zm));
+    TRY(check_product(fn, w0m, xm));
+    TRY(check_product(fn, w2m, zm));
+    TRY(check_bias(fn, b0_dev));
+    TRY(check_bias(fn, b2_dev));
+    if (w0m.rows % 2) return fail(T0B_ERR_INVALID, fn, "w0 needs gate and up rows in equal number");
+    if (zm.rows != xm.rows || zm.k != w0m.rows / 2 || zm.blk != w0m.blk)
+      return fail(T0B_ERR_INVALID, fn, "zq must have w0's format and shape [xq->rows, w0->rows / 2]");
+    TRY(check_plain(fn, "x", x_type, x_dev, ldx, xm.rows, xm.k));
+    TRY(check_plain(fn, "y", y_type, y_dev, ldy, xm.rows, w2m.rows));
+    DeviceScope dev(t0b_engine_device(e));
+    TRY(cuda_status(fn, dev.status));
+    const cudaStream_t st = (cudaStream_t)stream;
+    int *err = t0b_engine_fp4_err(e);
+    const Fp4Out hid{0, nullptr, 0, b0_dev, true, true, zm};
+    TRY(cuda_status(fn, t0b_launch_fp4_linear(w0m, x_type, x_dev, ldx, xm, hid, err, st)));
+    const Fp4Out out{y_type, y_dev, ldy, b2_dev, false, false, {}};
+    return cuda_status(fn, t0b_launch_fp4_gemm(w2m, zm, out, true, err, st));
+  });
 }
 
 extern "C" t0b_status t0b_fp4_sync(t0b_engine *e, void *stream) {
-  const char *fn = "t0b_fp4_sync";
-  if (!e) return fail(T0B_ERR_INVALID, fn, "engine is NULL");
-  DeviceScope dev(t0b_engine_device(e));
-  TRY(cuda_status(fn, dev.status));
-  const cudaStream_t st = (cudaStream_t)stream;
-  int *err = t0b_engine_fp4_err(e), herr = 0;
-  TRY(cuda_status(fn, cudaMemcpyAsync(&herr, err, sizeof(int), cudaMemcpyDeviceToHost, st)));
-  TRY(cuda_status(fn, cudaStreamSynchronize(st)));
-  if (!herr) return T0B_OK;
-  TRY(cuda_status(fn, cudaMemsetAsync(err, 0, sizeof(int), st)));
-  TRY(cuda_status(fn, cudaStreamSynchronize(st)));
-  char what[80];
-  snprintf(what, sizeof(what), "a kernel reported device error code %d", herr);
-  return fail(T0B_ERR_DEVICE, fn, what);
+  return guarded([&]() -> t0b_status {
+    const char *fn = "t0b_fp4_sync";
+    if (!e) return fail(T0B_ERR_INVALID, fn, "engine is NULL");
+    DeviceScope dev(t0b_engine_device(e));
+    TRY(cuda_status(fn, dev.status));
+    const cudaStream_t st = (cudaStream_t)stream;
+    int *err = t0b_engine_fp4_err(e), herr = 0;
+    TRY(cuda_status(fn, cudaMemcpyAsync(&herr, err, sizeof(int), cudaMemcpyDeviceToHost, st)));
+    TRY(cuda_status(fn, cudaStreamSynchronize(st)));
+    if (!herr) return T0B_OK;
+    TRY(cuda_status(fn, cudaMemsetAsync(err, 0, sizeof(int), st)));
+    TRY(cuda_status(fn, cudaStreamSynchronize(st)));
+    char what[80];
+    snprintf(what, sizeof(what), "a kernel reported device error code %d", herr);
+    return fail(T0B_ERR_DEVICE, fn, what);
+  });
 }

@@ -9,6 +9,9 @@ sum|xw|, plus half a step of the output type (2^-24, 2^-11, 2^-8 relative, and
 half the smallest float16 subnormal, 2^-25).  A gated product adds d(silu) <=
 1.1 dg, |silu(g)| <= |g| and 8 units of 2^-24 for exp, quotient and products.
 """
+import os
+import subprocess
+import sys
 import threading
 
 import numpy as np
@@ -178,7 +181,7 @@ def test_dequantize_every_byte(engine, fmt):
 SHAPES = [(1, 1, 1), (1, 128, 256), (1, 4096, 4096), (2, 16, 31), (3, 100, 1000), (8, 512, 512), (16, 129, 257), (17, 1536, 512),
           (19, 512, 2048), (31, 257, 96), (33, 1000, 1001), (64, 640, 1024), (65, 64, 64), (100, 1024, 512), (127, 128, 128),
           (128, 256, 256), (129, 257, 320), (200, 8, 5000), (256, 192, 63), (300, 1001, 1000), (333, 384, 4096), (513, 2048, 512),
-          (1000, 300, 128), (2100, 130, 96)]
+          (1000, 300, 128), (2100, 130, 96), (4, 128, 70000), (300, 260, 20000), (700, 64, 64), (1025, 33, 257)]
 
 
 @pytest.mark.parametrize("fmt", FMT)
@@ -216,7 +219,7 @@ def test_gemm_exact_sums(engine, fmt, m):
 
 
 @pytest.mark.parametrize("fmt", FMT)
-@pytest.mark.parametrize("m", [3, 200])
+@pytest.mark.parametrize("m", [3, 200, 900])
 def test_gemm_non_finite_blocks_stay_in_their_rows(engine, fmt, m):
     n, k = 150, 200
     xv, wv = rnd(1, m, k), rnd(2, n, k)
@@ -300,7 +303,8 @@ def test_glu_extreme_gates(engine):
 # ---------------------------------------------------- the operators together
 @pytest.mark.parametrize("fmt", FMT)
 @pytest.mark.parametrize("ty", ["f32", "f16", "bf16"])
-@pytest.mark.parametrize("m,n,k,pad", [(1, 512, 512, 0), (5, 100, 1001, 3), (19, 1536, 512, 0), (32, 1000, 64, 1), (150, 257, 200, 8)])
+@pytest.mark.parametrize("m,n,k,pad", [(1, 512, 512, 0), (5, 100, 1001, 3), (19, 1536, 512, 0), (32, 1000, 64, 1), (150, 257, 200, 8),
+                                       (64, 300, 256, 1), (63, 40, 2048, 0), (2, 64, 8192, 5), (700, 300, 130, 1)])
 def test_linear_is_quantize_and_gemm(engine, fmt, ty, m, n, k, pad):
     x = torch.from_numpy(rnd(m, m, k + pad)).to(DT[ty]).to(DEV)[:, :k]
     wq, w = mat_from(rnd(n, n, k, dev=0.05), fmt)
@@ -429,6 +433,27 @@ def test_offsets_past_32_bits(engine):
         fp4.gemm(engine, wq, m, g2)
         assert torch.equal(x[:, :80], g2)
         x.copy_(v)
+
+
+def _process(*args):
+    r = subprocess.run([sys.executable, os.path.join(os.path.dirname(__file__), "fp4_cases.py"), *args], capture_output=True,
+                       text=True, timeout=300)
+    assert r.returncode == 0, f"{args}: {r.stdout[-2000:]}\n{r.stderr[-4000:]}"
+
+
+def test_checked_build_matches_product_bit_for_bit(tmp_path):
+    """No index check of the checked build fails, and it computes the same bits."""
+    _process("product", str(tmp_path / "p.npz"))
+    _process("checked", str(tmp_path / "c.npz"))
+    a, b = np.load(tmp_path / "p.npz"), np.load(tmp_path / "c.npz")
+    assert sorted(a.files) == sorted(b.files) and len(a.files) == 96
+    for k in a.files:
+        assert np.isfinite(b[k]).all(), k
+        assert np.array_equal(a[k], b[k]), k
+
+
+def test_first_calls_of_a_process_can_be_captured():
+    _process("capture")
 
 
 # ---------------------------------------------------------------- refusals
