@@ -203,7 +203,7 @@ t0b_status t0b_qmatrix_sync(t0b_qmatrix *q, void *stream);
  *   T0B_FP4_MX  blocks of 32, scale = 2^(byte - 127), byte 255 = NaN;
  *               tensor_scale must be 1
  *   T0B_FP4_NV  blocks of 16, scale = an unsigned float with 4 exponent (bias
- *               7) and 3 mantissa bits, byte 127 = NaN; tensor_scale is any
+ *               7) and 3 mantissa bits, byte 127 = NaN, none above; tensor_scale is any
  *               positive normal number (a power of two in [2^-64, 2^64] where
  *               a call quantises, so that every rounding is decided exactly)
  *
@@ -273,7 +273,7 @@ t0b_status t0b_fp4_mlp(t0b_engine *e, const t0b_fp4 *w0, const t0b_fp4 *w2, int 
                        const t0b_fp4 *xq, const t0b_fp4 *zq, const float *b0_dev, const float *b2_dev, int y_type,
                        void *y_dev, int64_t ldy, void *stream);
 /* Wait for `stream` and report any kernel-side error of the engine's 4-bit
- * operators since the last call. */
+ * operators since the last call (not while `stream` is being captured). */
 t0b_status t0b_fp4_sync(t0b_engine *e, void *stream);
 
 /* ---- bounded-wait self-test (no reference counterpart; a diagnostic) ----

@@ -101,6 +101,7 @@ t0b_status check_product(const char *fn, const Fp4Mat &w, const Fp4Mat &x) {
 
 t0b_status cuda_status(const char *fn, cudaError_t e) {
   if (e == cudaSuccess) return T0B_OK;
+  cudaGetLastError();  // reported here: not left for the caller's next check
   return fail(T0B_ERR_CUDA, fn, cudaGetErrorString(e));
 }
 

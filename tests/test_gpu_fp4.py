@@ -234,6 +234,24 @@ def test_gemm_non_finite_blocks_stay_in_their_rows(engine, fmt, m):
     assert np.isnan(got[bad]).all() and np.isfinite(got[~bad]).all()
 
 
+@pytest.mark.parametrize("m", [5, 600])
+@pytest.mark.parametrize("fmt", FMT)
+def test_gemm_every_scale_byte(engine, fmt, m):
+    """Random codes under every finite scale byte (mx: those whose products stay normal), subnormal scales among them."""
+    n, k = 140, 256
+    rng = np.random.default_rng(m)
+    mats = []
+    for rows in (m, n):
+        code = rng.integers(0, 16, (rows, k)).astype(np.uint8)
+        byte = rng.integers(*((70, 185) if fmt == "mx" else (0, 127)), (rows, k // O.BLOCK[fmt])).astype(np.uint8)
+        c, s = O.pack(byte, code, fmt)
+        mats.append((fp4.Fp4Matrix(fmt, rows, k, torch.from_numpy(c).to(DEV), torch.from_numpy(s).to(DEV)), O.values(byte, code, fmt)))
+    y = torch.empty((m, n), device=DEV)
+    fp4.gemm(engine, mats[1][0], mats[0][0], y)
+    (_, x), (_, w) = mats
+    check_close(y, x @ w.T, sum_bound(x, w) + 2.0 ** -24 * np.abs(x @ w.T))
+
+
 def test_gemm_wide_range_of_scales(engine):
     """Blocks of very different scale, in rows of their own: the result follows the largest."""
     m, n, k = 40, 130, 512
