@@ -412,6 +412,20 @@ T0B_DEV void tmem_ld_wait(uint32_t *r) {
                  "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
                  "+r"(r[30]), "+r"(r[31])::"memory");
 }
+// 16 accumulator columns of this thread's lane; used after the wait on them.
+T0B_DEV void tmem_ld16(uint32_t addr, uint32_t *r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(addr));
+}
+T0B_DEV void tmem_ld_wait16(uint32_t *r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]),
+                 "+r"(r[15])::"memory");
+}
 T0B_DEV void tma_load_3d_pair(void *dst, const void *tmap, uint32_t bar_cl, int x, int y, int z) {
   asm volatile(
       "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, "
@@ -495,8 +509,9 @@ struct Fp4Args {
 // else; it works while the next tile is multiplied.
 // Bound by the tensor cores and, in a long run, by the power limit: 8192 x
 // 8192 x 8192 MX 170 us, NV 176 us (6.5 and 6.2 PFLOP/s); short K by the
-// epilogue: 65,536 x 1024 x 1024 to f32 54 us (268 MB written), gated and
-// quantised 32,768 x 4096 x 1024 132 us (two MUFU operations a value).
+// epilogue: 65,536 x 1024 x 1024 to f32 56 us (268 MB written), gated and
+// quantised 32,768 x 4096 x 1024 MX 129 us, NV 143 us (two MUFU operations a
+// value).
 // Measured and not kept: three accumulators of 128 columns in turn (equal,
 // NV 9 % slower: the MMA warp issues twice the MMAs); the scale copies by
 // another warp (8 % slower: one more hop a stage); token tiles fastest (equal).
@@ -554,16 +569,12 @@ T0B_DEV void store_quant32(const Fp4Mat &q, int r, int c0, float *v) {
 }
 
 // 32 rows x 64 bytes of the result, one row per lane, columns c0 .. : through
-// the warp's staging buffer (64-byte swizzle) and out by a TMA store, or, where
-// the result's rows are not 16-byte aligned, element by element along the rows.
+// the warp's staging buffer (64-byte swizzle) and out by a TMA store.
 template <int TY>
 T0B_DEV void store_rows(const Fp4Args &p, const void *tm_y, uint8_t *stg, int row0, int c0, const float *v) {
   using T = typename Plain<TY>::T;
-  constexpr int W = 64 / sizeof(T);
   const int lane = threadIdx.x & 31;
-  if (p.vec) {
-    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-  }
+  if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
   __syncwarp();  // the buffer has been read
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -573,42 +584,56 @@ T0B_DEV void store_rows(const Fp4Args &p, const void *tm_y, uint8_t *stg, int ro
     for (int j = 0; j < PER; ++j) t[j] = Plain<TY>::put(v[i * PER + j]);
     *reinterpret_cast<uint4 *>(stg + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4)) = *reinterpret_cast<const uint4 *>(t);
   }
-  if (p.vec) {
-    fence_proxy_async_smem();
-    __syncwarp();
-    if (lane == 0) {
-      if (row0 < p.M && c0 < p.n && T0B_CHECK_TMA(c0, (int)sizeof(T), row0, p.err)) tma_store_2d(tm_y, stg, c0, row0);
-      bulk_commit();
-    }
-  } else {
-    __syncwarp();
-    // half a warp a row, 4-byte words: 16-bit values in pairs, single ones at the ends
-    auto at = [&](int r, int c) {
-      return *reinterpret_cast<const T *>(stg + r * 64 + (((c * (int)sizeof(T) >> 4) ^ ((r >> 1) & 3)) << 4) + (c * (int)sizeof(T) & 15));
-    };
-    const int n = min(W, p.n - c0), hl = lane & 15;
-    if (n <= 0) return;
-    T *y = reinterpret_cast<T *>(p.y) + (int64_t)(row0 + (lane >> 4)) * p.ld + c0;
-#pragma unroll 4
-    for (int r = lane >> 4; r < 32; r += 2, y += 2 * p.ld) {
-      if (row0 + r >= p.M) break;
-      if constexpr (sizeof(T) == 4) {
-        if (hl < n) y[hl] = at(r, hl);
-      } else {
-        const int e = 2 * hl - (int)((uintptr_t)y >> 1 & 1);
-        if (e >= 0 && e + 1 < n) {
-          const T t[2] = {at(r, e), at(r, e + 1)};
-          *reinterpret_cast<uint32_t *>(y + e) = *reinterpret_cast<const uint32_t *>(t);
-        } else if (e < n) {
-          y[e < 0 ? 0 : e] = at(r, e < 0 ? 0 : e);
-        }
-      }
-    }
-    if constexpr (sizeof(T) == 2) {  // the last value of rows that start in the middle of a word, one row a lane
-      y = reinterpret_cast<T *>(p.y) + (int64_t)(row0 + lane) * p.ld + c0;
-      if (n == W && row0 + lane < p.M && ((uintptr_t)y >> 1 & 1)) y[W - 1] = at(lane, W - 1);
-    }
+  fence_proxy_async_smem();
+  __syncwarp();
+  if (lane == 0) {
+    if (row0 < p.M && c0 < p.n && T0B_CHECK_TMA(c0, (int)sizeof(T), row0, p.err)) tma_store_2d(tm_y, stg, c0, row0);
+    bulk_commit();
   }
+}
+
+// The same where the result's rows are not 16-byte aligned: the four warps h of
+// a lane quarter bring their 64 bytes a row together in the quarter's 8 KB
+// (16-byte pieces swizzled by the row), and each writes 8 of the 32 rows, 256
+// bytes of a row at a time: the sectors at both ends are written in part, and
+// that is what unaligned rows cost.  32,768 x 4001 x 1024 to bf16 123 us, to
+// f32 187 us; with 64 bytes of a row at a time 214 and 309 us.
+T0B_DEV void quarter_sync(int q) { asm volatile("bar.sync %0, 128;" ::"r"(2 + q) : "memory"); }
+template <int TY>
+T0B_DEV void store_rows_unaligned(const Fp4Args &p, uint8_t *quarter, int q, int h, int row0, int c0, const float *v) {
+  using T = typename Plain<TY>::T;
+  constexpr int W = 256 / sizeof(T), PER = 16 / sizeof(T);  // columns of the four warps
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    alignas(16) T t[PER];
+#pragma unroll
+    for (int j = 0; j < PER; ++j) t[j] = Plain<TY>::put(v[i * PER + j]);
+    *reinterpret_cast<uint4 *>(quarter + lane * 256 + (((4 * h + i) ^ (lane & 15)) << 4)) = *reinterpret_cast<const uint4 *>(t);
+  }
+  quarter_sync(q);
+  const int first = c0 - W / 4 * h, n = p.n - first;
+  const int rows = min(8, p.M - row0 - 8 * h);
+  T *y = reinterpret_cast<T *>(p.y) + (int64_t)(row0 + 8 * h) * p.ld + first + lane;
+  constexpr int B = 2 * sizeof(T);  // rows at a time
+#pragma unroll 1
+  for (int r0 = 0; r0 < rows; r0 += B) {
+    T t[B][W / 32];
+#pragma unroll
+    for (int r = 0; r < B; ++r)
+#pragma unroll
+      for (int i = 0; i < W / 32; ++i) {
+        const int c = lane + 32 * i, row = 8 * h + r0 + r;
+        t[r][i] = *reinterpret_cast<const T *>(quarter + row * 256 + (((c / PER) ^ (row & 15)) << 4) + c % PER * (int)sizeof(T));
+      }
+#pragma unroll
+    for (int r = 0; r < B; ++r, y += p.ld)
+      if (r0 + r < rows)
+#pragma unroll
+        for (int i = 0; i < W / 32; ++i)
+          if (lane + 32 * i < n) y[32 * i] = t[r][i];
+  }
+  quarter_sync(q);
 }
 
 // TY: result type, or -1 for the 4-bit result of a gated product.
@@ -782,41 +807,62 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
   } else {
     // ------------------------------------------------------------ epilogue (both CTAs)
     setmaxnreg_inc<PAIR_REGS_EPI>();
-    const int q = warp & 3, h = (warp - 4) >> 2;  // lane quarter, 64 columns (gated: 32 gate, 32 up)
-    uint8_t *stg = smem + C::OFF_STG + (warp - 4) * 2048;
+    // Lane quarter q; of the tile's columns this warp has W from W h on, and
+    // every 4 W further (W: 64 bytes of the result), gated the up ones too.
+    constexpr int OT = TY < 0 ? TY_F32 : TY, W = TY == TY_F32 ? 16 : 32, N = (GLU ? 32 : 64) / W;
+    const int q = warp & 3, h = (warp - 4) >> 2;
+    uint8_t *stg = smem + C::OFF_STG + (4 * q + h) * 2048;
     float *sb = reinterpret_cast<float *>(smem + C::OFF_BIAS) + (warp - 4) * 64;
     uint32_t it = 0;
     for (int tile = pair; tile < p.n_tiles; tile += npairs, ++it) {
       const int nt = tile % p.n_tiles_n, m0 = tile / p.n_tiles_n * 256 + 128 * (int)rank;
+      const int n0 = nt * (GLU ? 128 : 256);
       // this warp's 64 biases (gated: 32 gate, 32 up)
       __syncwarp();
-      {
-        const int c0 = GLU ? nt * 128 + 32 * h + lane : nt * 256 + 64 * h + lane, c1 = GLU ? c0 : c0 + 32;
-        sb[lane] = p.bias && c0 < p.n ? p.bias[c0] : 0.0f;
-        sb[32 + lane] = p.bias && c1 < p.n ? p.bias[GLU ? p.n + c1 : c1] : 0.0f;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int j = GLU ? lane : 32 * i + lane, c = n0 + W * h + j / W * 4 * W + j % W;
+        sb[32 * i + lane] = p.bias && c < p.n ? p.bias[GLU && i ? p.n + c : c] : 0.0f;
       }
       __syncwarp();
       const int row0 = m0 + 32 * q;
-      const uint32_t trow = tmem + ((uint32_t)(32 * q) << 16);
+      const uint32_t trow = tmem + ((uint32_t)(32 * q) << 16) + W * h;
       bool have = mbar_wait(acc_full, it & 1, p.err, T0B_DEVERR_WAIT_ACC, abort_flag) && !*abort_flag;
       have = __all_sync(0xFFFFFFFFu, have);
       tc_fence_after();
       uint32_t r[2][32];
       if (have) {
-        tmem_ld32(trow + (GLU ? 32 : 64) * h, r[0]);
-        tmem_ld32(trow + (GLU ? 128 + 32 * h : 64 * h + 32), r[1]);
+        if constexpr (W == 32) {
+          tmem_ld32(trow, r[0]);
+          tmem_ld32(trow + 128, r[1]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) tmem_ld16(trow + 64 * i, r[i / 2] + 16 * (i % 2));
+        }
         tmem_ld_wait(r[0]);
         tmem_ld_wait(r[1]);
       }
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(lead(acc_empty));
+      if (TY >= 0 && !p.vec) {  // the quarter's warps go on together or not at all
+        int all;
+        asm volatile("{\n .reg .pred a, b;\n setp.ne.b32 a, %1, 0;\n barrier.cta.red.and.pred b, %2, 128, a;\n selp.b32 %0, 1, 0, b;\n}"
+                     : "=r"(all)
+                     : "r"((int)have), "r"(2 + q)
+                     : "memory");
+        have = all;
+      }
       if (!have) continue;
-      constexpr int OT = TY < 0 ? TY_F32 : TY, W = OT == TY_F32 ? 16 : 32;
+      auto store = [&](int i, const float *v) {
+        if (p.vec)
+          store_rows<OT>(p, &tm_y, stg, row0, n0 + W * h + 4 * W * i, v);
+        else
+          store_rows_unaligned<OT>(p, smem + C::OFF_STG + q * 8192, q, h, row0, n0 + W * h + 4 * W * i, v);
+      };
       if constexpr (!GLU) {
 #pragma unroll
-        for (int i = 0; i < 64 / W; ++i) {
-          const int c0 = 64 * h + W * i;
+        for (int i = 0; i < N; ++i) {
           float v[W];
 #pragma unroll
           for (int j = 0; j < W; j += 4) {
@@ -827,10 +873,9 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
             v[j + 2] = fmaf(__uint_as_float(a[2]), p.alpha, b.z);
             v[j + 3] = fmaf(__uint_as_float(a[3]), p.alpha, b.w);
           }
-          store_rows<OT>(p, &tm_y, stg, row0, nt * 256 + c0, v);
+          store(i, v);
         }
       } else {
-        const int c0 = 32 * h, f0 = nt * 128 + c0;
         const F2 alpha(p.alpha, p.alpha);
         float *g = reinterpret_cast<float *>(r[0]), *u = reinterpret_cast<float *>(r[1]), *v = g;
 #pragma unroll
@@ -850,9 +895,9 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
         }
         if constexpr (TY >= 0) {
 #pragma unroll
-          for (int i = 0; i < 32 / W; ++i) store_rows<OT>(p, &tm_y, stg, row0, f0 + W * i, v + W * i);
+          for (int i = 0; i < N; ++i) store(i, v + W * i);
         } else {
-          store_quant32<NV>(p.q, row0 + lane, f0, v);
+          store_quant32<NV>(p.q, row0 + lane, n0 + 32 * h, v);
         }
       }
     }
@@ -925,20 +970,6 @@ T0B_DEV void quantize_lanes(const Fp4Mat &q, int r, int c0, float v) {
     *reinterpret_cast<uint32_t *>(q.codes + r * code_pitch(q.k) + (c0 + lane) / 2) = w;
 }
 
-// 16 accumulator columns of this thread's lane; used after the wait on them.
-T0B_DEV void tmem_ld16(uint32_t addr, uint32_t *r) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(addr));
-}
-T0B_DEV void tmem_ld_wait16(uint32_t *r) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
-                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]),
-                 "+r"(r[15])::"memory");
-}
 T0B_DEV void scale_cp(uint32_t taddr, uint64_t desc) {
   asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
 }
