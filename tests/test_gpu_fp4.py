@@ -432,6 +432,123 @@ def test_two_threads(engine):
     assert not bad
 
 
+@pytest.mark.parametrize("fmt", FMT)
+@pytest.mark.parametrize("m", [6, 40, 300])
+def test_linear_and_mlp_of_empty_and_non_finite_rows(engine, fmt, m):
+    """Rows of zeros, of one value, with a NaN or an infinity, very large and very small ones: as by the parts."""
+    k, f = 300, 200
+    xv = rnd(m, m, k).astype(np.float32)
+    xv[0], xv[1], xv[2, 7], xv[3, 299], xv[4] = 0, -0.0, np.nan, -np.inf, 1e-38
+    xv[5] *= 2.0 ** 60
+    x = torch.from_numpy(xv).to(DEV)
+    w0, _ = mat_from(rnd(1, 2 * f, k, dev=0.1), fmt)
+    w2, _ = mat_from(rnd(2, k, f, dev=0.1), fmt)
+    y, h, y2 = torch.empty((m, k), device=DEV), torch.empty((m, 2 * f), device=DEV), torch.empty((m, k), device=DEV)
+    fp4.mlp(engine, w0, w2, x, empty(fmt, m, k), empty(fmt, m, f), y)
+    fp4.linear(engine, w0, x, empty(fmt, m, k), h)
+    xq = fp4.quantize(engine, x, empty(fmt, m, k))
+    check_matrix(xq, xv.astype(np.float64))
+    fp4.gemm(engine, w2, fp4.glu(engine, w0, xq, empty(fmt, m, f)), y2)
+    h2 = fp4.gemm(engine, w0, xq, torch.empty_like(h))
+    fp4.sync(engine)
+    for a, b in ((y, y2), (h, h2)):
+        assert torch.equal(a.isnan(), b.isnan()) and torch.equal(a.nan_to_num(), b.nan_to_num())
+    assert bool((h[:2] == 0).all()) and bool((y[:2] == 0).all())
+    assert bool(h[2:4].isnan().all()) and bool(y[2:4].isnan().all()) and bool(h[4:].isfinite().all())
+
+
+def test_kernels_of_every_kind_at_once(engine):
+    """Products in clusters of several sizes, on CTA pairs and fused, from four streams at the same time."""
+    jobs = []
+    for i, (m, n, k, fmt) in enumerate([(1, 512, 4096, "nv"), (40, 1024, 2048, "mx"), (700, 2048, 512, "nv"), (19, 4096, 1024, "mx"),
+                                        (100, 130, 8192, "nv"), (2000, 512, 256, "mx"), (64, 512, 512, "nv"), (300, 4000, 300, "mx")]):
+        w, _ = mat_from(rnd(i, 2 * n, k, dev=0.1), fmt)
+        x = torch.from_numpy(rnd(50 + i, m, k).astype(np.float32)).to(DEV)
+        jobs.append((w, x, fmt, m, n, k))
+
+    def run(job, y, z):
+        w, x, fmt, m, n, k = job
+        fp4.linear(engine, w, x, empty(fmt, m, k), y)
+        fp4.glu(engine, w, fp4.quantize(engine, x, empty(fmt, m, k)), z)
+
+    outs = [[(torch.empty((j[3], 2 * j[4]), device=DEV), torch.empty((j[3], j[4]), device=DEV)) for j in jobs] for _ in range(5)]
+    for j, o in zip(jobs, outs[4]):
+        run(j, *o)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    for rep in range(10):
+        for i in range(len(jobs)):
+            for s in range(4):
+                with torch.cuda.stream(streams[s]):
+                    a = (i + 2 * s) % len(jobs)
+                    run(jobs[a], *outs[s][a])
+    torch.cuda.synchronize()
+    fp4.sync(engine)
+    for s in range(4):
+        for (y, z), (y0, z0) in zip(outs[s], outs[4]):
+            assert torch.equal(y, y0) and torch.equal(z, z0)
+
+
+def test_capture_across_streams(engine):
+    """A captured fork and join: operators that follow another stream's work by events."""
+    m, f, k = 33, 256, 128
+    w0, _ = mat_from(rnd(1, 2 * f, k, dev=0.1), "mx")
+    x = torch.from_numpy(rnd(2, m, k).astype(np.float32)).to(DEV)
+    xq, xq2 = empty("mx", m, k), empty("mx", m, k)
+    z, y, total = torch.empty((m, f), device=DEV), torch.empty((m, 2 * f), device=DEV), torch.empty((m, f), device=DEV)
+
+    def run(s1, s2):
+        with torch.cuda.stream(s1):
+            x.mul_(2.0)
+            fp4.quantize(engine, x, xq)
+        s2.wait_stream(s1)
+        with torch.cuda.stream(s2):
+            fp4.gemm(engine, w0, xq, y)
+        with torch.cuda.stream(s1):
+            fp4.glu(engine, w0, xq, z)
+        s1.wait_stream(s2)
+        with torch.cuda.stream(s1):
+            fp4.quantize(engine, x, xq2)
+            torch.add(z, y[:, :f], out=total)
+
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    run(s1, s2)
+    torch.cuda.synchronize()
+    want, x0 = total.clone(), x.clone()
+    g = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g, stream=s1):
+        run(s1, s2)
+    for _ in range(3):
+        x.copy_(x0 / 2)
+        total.fill_(float("nan"))
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(total, want) and torch.equal(xq.codes, xq2.codes)
+    fp4.sync(engine)
+
+
+@pytest.mark.parametrize("fmt", FMT)
+def test_many_rows_and_many_columns(engine, fmt):
+    k, n = 48, 20
+    base = torch.from_numpy(rnd(1, 1000, k).astype(np.float32)).to(DEV)
+    x = base.repeat(2101, 1)  # 2,101,000 tokens
+    w, _ = mat_from(rnd(2, n, k), fmt)
+    xq = fp4.quantize(engine, x, empty(fmt, len(x), k))
+    y = fp4.gemm(engine, w, xq, torch.empty((len(x), n), dtype=torch.bfloat16, device=DEV))
+    small = fp4.gemm(engine, w, fp4.quantize(engine, base, empty(fmt, 1000, k)), torch.empty((1000, n), dtype=torch.bfloat16, device=DEV))
+    assert torch.equal(y.view(2101, 1000, n), small.expand(2101, 1000, n))
+    back = fp4.dequantize(engine, xq, torch.empty_like(x))
+    assert torch.equal(back.view(2101, 1000, k), back[:1000].expand(2101, 1000, k))
+    # the same matrices the other way round: 2,101,000 weight rows, a few tokens and a few hundred
+    for m in (3, 300):
+        t = fp4.quantize(engine, base[:m].contiguous(), empty(fmt, m, k))
+        wide = fp4.gemm(engine, xq, t, torch.empty((m, len(x)), dtype=torch.bfloat16, device=DEV))
+        assert torch.equal(wide.view(m, 2101, 1000), wide[:, None, :1000].expand(m, 2101, 1000))
+
+
 def test_offsets_past_32_bits(engine):
     """Rows of x and y that lie more than 2^32 bytes into their buffers."""
     rows, k, ld = 2200, 96, 1 << 20
