@@ -174,8 +174,8 @@ T0B_DEV uint32_t quantize8(const BlockScale<NV> &s, const float *v) {
 // loads are in flight per lane, and a tile's 16 bytes of scales are written
 // together.  A block spans two (NV) or four lanes; its largest magnitude is
 // joined by shuffles, the scale words by a 4 x 4 byte transposition.
-// Bound by HBM: 65,536 x 1024 bf16 in 31.8 us (MX) and 33.9 us (NV), 170 MB =
-// 5.3 and 5.0 TB/s; f32 6.2 TB/s.  One thread per block took 535 us for this
+// Bound by HBM: 65,536 x 1024 bf16 in 31.9 us (MX) and 32.1 us (NV), 170 MB =
+// 5.3 TB/s; f32 6.2 TB/s.  One thread per block took 535 us for this
 // and the way back.
 constexpr int QT_WARPS = 8;
 constexpr int QT_CHUNKS = 4;  // 65,536 x 1024 bf16: 39 us with 1, 35 with 2, 32 with 4 and 8
@@ -209,7 +209,7 @@ struct Raw8 {
   }
 };
 
-// LPR: lanes along a row, a scale tile's (8 or 16) or 32.
+// LPR: lanes along a row, 8 (one NV scale tile), 16 or 32.
 // A warp goes through `chunks` such pieces along its rows and fetches the next
 // one before it works on the present one.
 template <int TY, bool NV, int LPR>
@@ -222,23 +222,32 @@ __global__ void __launch_bounds__(32 * QT_WARPS)
   const int r0 = blockIdx.x * (QT_WARPS * RPW) + (threadIdx.x >> 5) * RPW + lane / LPR;  // counts 32 rows of each group
   const int group = r0 >> 5, r = group * 128 + (r0 & 31);
   int k0 = (blockIdx.y * chunks * LPR + lane % LPR) * 8;
+  const int live = min(4, (q.rows - r + 31) / 32);  // of this lane's four rows
+  const size_t pitch = code_pitch(q.k);
+  const typename Plain<TY>::T *row = x + r * ldx;
+  uint8_t *codes = q.codes + r * pitch + k0 / 2;
+  const int t0 = k0 / (4 * BLK), b = lane / LB % 4;
+  uint8_t *scales = q.scales + ((size_t)group * kt + t0) * 512 + (r & 31) * 16 + 4 * b;
+  const uint32_t sel1 = b & 1 ? 0x3715 : 0x6240, sel2 = b & 2 ? 0x3276 : 0x5410;
+  const bool writes_scales = lane % LB == 0 && group < (q.rows + 127) / 128;
   pdl_wait();
   pdl_launch_dependents();
   Raw8<TY> next[4];
   auto fetch = [&](int k) {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      if (r + 32 * i < q.rows)
-        next[i].load(x + (r + 32 * i) * ldx, k, q.k, vec);
+      if (i < live)
+        next[i].load(row + 32 * i * ldx, k, q.k, vec);
       else
         next[i].zero();
   };
   fetch(k0);
-  for (int c = 0; c < chunks; ++c, k0 += 8 * LPR) {
+  for (int c = 0; c < chunks; ++c) {
     Raw8<TY> raw[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) raw[i] = next[i];
     if (c + 1 < chunks) fetch(k0 + 8 * LPR);
+    const int rows = k0 / 2 < (int)pitch ? live : 0;
     uint32_t sc = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -249,16 +258,15 @@ __global__ void __launch_bounds__(32 * QT_WARPS)
       for (int o = 1; o < LB; o *= 2) top = absmax(top, __shfl_xor_sync(0xFFFFFFFFu, top, o), 0.0f);
       const BlockScale<NV> s(__float_as_uint(top), q);
       sc |= s.byte << (8 * i);
-      if (r + 32 * i < q.rows && k0 / 2 < (int)code_pitch(q.k))
-        *reinterpret_cast<uint32_t *>(q.codes + (r + 32 * i) * code_pitch(q.k) + k0 / 2) = quantize8<NV>(s, v);
+      if (i < rows) *reinterpret_cast<uint32_t *>(codes + 32 * i * pitch) = quantize8<NV>(s, v);
     }
     // sc: one block of four rows; the tile's words are four blocks of one row
-    const int b = lane / LB % 4;
-    sc = __byte_perm(sc, __shfl_xor_sync(0xFFFFFFFFu, sc, LB), b & 1 ? 0x3715 : 0x6240);
-    sc = __byte_perm(sc, __shfl_xor_sync(0xFFFFFFFFu, sc, 2 * LB), b & 2 ? 0x3276 : 0x5410);
-    const int t = k0 / (4 * BLK);
-    if (lane % LB == 0 && t < kt && group < (q.rows + 127) / 128)
-      *reinterpret_cast<uint32_t *>(q.scales + ((size_t)group * kt + t) * 512 + (r & 31) * 16 + 4 * b) = sc;
+    sc = __byte_perm(sc, __shfl_xor_sync(0xFFFFFFFFu, sc, LB), sel1);
+    sc = __byte_perm(sc, __shfl_xor_sync(0xFFFFFFFFu, sc, 2 * LB), sel2);
+    if (writes_scales && k0 < 4 * BLK * kt) *reinterpret_cast<uint32_t *>(scales) = sc;
+    k0 += 8 * LPR;
+    codes += 4 * LPR;
+    scales += 512 * (8 * LPR / (4 * BLK));
   }
 }
 
@@ -1408,7 +1416,8 @@ SplitPlan split_plan(bool glu, int M, int n, int K, int most, int sms) {
   const int64_t tiles = (int64_t)q.rt * ((M + q.NT - 1) / q.NT);
   const int S = (K + 255) / 256;
   // clusters have to fit the GPCs: of 8 CTAs not more than two thirds of the
-  // SMs can be used at once
+  // SMs can be used at once (1024 x 4096, 256 tokens in tiles of 128: 128 CTAs
+  // in clusters of 8 13.5 us, 96 in clusters of 4 for 384 tokens 8.4 us)
   int cs = 1;
   while (cs < SPLIT_MAX_CLUSTER && tiles * cs * 2 <= (cs == 4 ? sms * 2 / 3 : sms * 7 / 8) && S >= cs * 2) cs *= 2;
   q.SL = (S + cs - 1) / cs;
@@ -1551,25 +1560,31 @@ cudaError_t gemm_fmt(const Fp4Mat &w, const Fp4Mat &x, const Fp4Out &out, const 
   return gemm_ty<NV, TY_BF16>(w, x, out, p, st);
 }
 
-// Rows of one scale tile's width get the lanes of one tile, longer ones a warp.
+// Lanes along a row: those of one scale tile (8 NV, 16 MX) for rows no wider,
+// 16 up to 128 values, else the warp.  65,536 x 16 f16 quantised in 4.2 us (NV)
+// and 6.0 us (MX), with the whole warp along a row 11.2 and 10.5 us.
 template <int TY, bool NV, bool QUANT>
 cudaError_t convert(const void *x, int64_t ld, const Fp4Mat &q, cudaStream_t st) {
   using T = typename Plain<TY>::T;
-  constexpr int SHORT = NV ? 8 : 16;
+  constexpr int TILE = NV ? 8 : 16;
   // expansion writes 32 bytes of f32 at once
-  const bool vec = QUANT || TY != TY_F32 ? rows_aligned(x, ld, TY) : ((uintptr_t)x | (uint64_t)ld * 4) % 32 == 0, narrow = q.k <= 8 * SHORT;
-  const int lpr = narrow ? SHORT : 32, row_warps = (q.rows + 127) / 128 * lpr;  // of 32 / lpr rows, 32 rows a group
-  const int width = QUANT ? (q.k + 8 * SHORT - 1) / (8 * SHORT) * (8 * SHORT) : q.k;  // whole scale tiles
+  const bool vec = QUANT || TY != TY_F32 ? rows_aligned(x, ld, TY) : ((uintptr_t)x | (uint64_t)ld * 4) % 32 == 0;
+  const int lpr = q.k <= 8 * TILE ? TILE : q.k <= 128 ? 16 : 32;
+  const int row_warps = (q.rows + 127) / 128 * lpr;  // of 32 / lpr rows, 32 rows a group
+  const int width = QUANT ? (q.k + 8 * TILE - 1) / (8 * TILE) * (8 * TILE) : q.k;  // whole scale tiles
   dim3 grid((row_warps + QT_WARPS - 1) / QT_WARPS, (width + 8 * lpr - 1) / (8 * lpr));
   if constexpr (QUANT) {
     // pieces of a row one after the other in a warp, as long as two waves of CTAs remain
     int chunks = 1;
     while (chunks < QT_CHUNKS && grid.y > 1 && (int64_t)grid.x * grid.y > 2 * 4 * sm_count()) chunks *= 2, grid.y = (grid.y + 1) / 2;
-    return narrow ? launch(fp4_quantize_kernel<TY, NV, SHORT>, grid, 32 * QT_WARPS, st, (const T *)x, ld, q, vec, chunks)
-                  : launch(fp4_quantize_kernel<TY, NV, 32>, grid, 32 * QT_WARPS, st, (const T *)x, ld, q, vec, chunks);
-  } else
-    return narrow ? launch(fp4_dequantize_kernel<TY, NV, SHORT>, grid, 32 * QT_WARPS, st, q, (T *)x, ld, vec)
-                  : launch(fp4_dequantize_kernel<TY, NV, 32>, grid, 32 * QT_WARPS, st, q, (T *)x, ld, vec);
+    auto k = lpr == TILE ? fp4_quantize_kernel<TY, NV, TILE> : lpr == 16 ? fp4_quantize_kernel<TY, NV, 16> : fp4_quantize_kernel<TY, NV, 32>;
+    return launch(k, grid, 32 * QT_WARPS, st, (const T *)x, ld, q, vec, chunks);
+  } else {
+    auto k = lpr == TILE ? fp4_dequantize_kernel<TY, NV, TILE>
+             : lpr == 16 ? fp4_dequantize_kernel<TY, NV, 16>
+                         : fp4_dequantize_kernel<TY, NV, 32>;
+    return launch(k, grid, 32 * QT_WARPS, st, q, (T *)x, ld, vec);
+  }
 }
 template <bool NV, bool QUANT>
 cudaError_t convert_ty(int type, const void *x, int64_t ld, const Fp4Mat &q, cudaStream_t st) {

@@ -84,7 +84,8 @@ def check_matrix(m, x):
 @pytest.mark.parametrize("fmt", FMT)
 @pytest.mark.parametrize("ty", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("rows,k,pad,shift", [(1, 1, 0, 0), (1, 1024, 0, 0), (3, 15, 0, 0), (5, 17, 3, 1), (128, 64, 0, 0),
-                                              (129, 65, 0, 0), (33, 1001, 7, 0), (300, 512, 8, 8), (257, 256, 1, 0), (2, 8192, 0, 0)])
+                                              (129, 65, 0, 0), (33, 1001, 7, 0), (300, 512, 8, 8), (257, 256, 1, 0), (2, 8192, 0, 0),
+                                              (140, 100, 0, 0), (33, 128, 4, 0)])
 def test_quantize(engine, fmt, ty, rows, k, pad, shift):
     buf = torch.from_numpy(rnd(rows * 7 + k, rows * (k + pad) + shift, dev=3.0)).to(DT[ty]).to(DEV)
     x = buf[shift:].view(rows, k + pad)[:, :k]
@@ -153,7 +154,8 @@ def test_quantize_every_16_bit_value(engine, ty, fmt):
 
 @pytest.mark.parametrize("fmt", FMT)
 @pytest.mark.parametrize("ty", ["f32", "f16", "bf16"])
-@pytest.mark.parametrize("rows,k,pad", [(1, 1, 0), (1, 1024, 0), (7, 33, 2), (130, 1001, 1), (129, 256, 8), (64, 48, 0)])
+@pytest.mark.parametrize("rows,k,pad", [(1, 1, 0), (1, 1024, 0), (7, 33, 2), (130, 1001, 1), (129, 256, 8), (64, 48, 0), (140, 100, 3),
+                                        (33, 128, 0)])
 def test_dequantize(engine, fmt, ty, rows, k, pad):
     m, v = mat_from(rnd(rows + k, rows, k), fmt)
     y = torch.full((rows, k + pad), 77.0, dtype=DT[ty], device=DEV)
