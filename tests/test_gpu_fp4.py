@@ -179,6 +179,27 @@ def test_dequantize_every_byte(engine, fmt):
     assert np.array_equal(y.cpu().numpy(), ref, equal_nan=True)
 
 
+@pytest.mark.parametrize("m", [7, 700])
+def test_any_tensor_scale_in_expansion_and_product(engine, m):
+    """Scales of matrices made elsewhere need not be powers of two: one f32 rounding in expansion, a factor in products."""
+    n, k, ts = 70, 96, (np.float32(0.3), np.float32(1.7e-5))
+    mats = []
+    for rows, t in zip((m, n), ts):
+        byte, code = O.quantize(rnd(rows, rows, k), "nv", 2.0 ** -6)
+        c, s = O.pack(byte, code, "nv")
+        mats.append((fp4.Fp4Matrix("nv", rows, k, torch.from_numpy(c).to(DEV), torch.from_numpy(s).to(DEV), float(t)),
+                     O.values(byte, code, "nv", np.float64(t))))
+    (xq, x), (wq, w) = mats
+    y = fp4.dequantize(engine, xq, torch.empty((m, k), device=DEV))
+    assert np.array_equal(y.cpu().numpy(), x.astype(np.float32))
+    p = fp4.gemm(engine, wq, xq, torch.empty((m, n), device=DEV))
+    # the factors' f32 product and the multiplication by it: two half steps
+    check_close(p, x @ w.T, sum_bound(x, w) + 2 * 2.0 ** -24 * np.abs(x @ w.T))
+    again = fp4.gemm(engine, xq, xq, torch.empty((m, m), device=DEV))  # one matrix on both sides
+    check_close(again, x @ x.T, sum_bound(x, x) + 2 * 2.0 ** -24 * np.abs(x @ x.T))
+    assert torch.equal(again, again.T)
+
+
 # ----------------------------------------------------------------- product
 SHAPES = [(1, 1, 1), (1, 128, 256), (1, 4096, 4096), (2, 16, 31), (3, 100, 1000), (8, 512, 512), (16, 129, 257), (17, 1536, 512),
           (19, 512, 2048), (31, 257, 96), (33, 1000, 1001), (64, 640, 1024), (65, 64, 64), (100, 1024, 512), (127, 128, 128),
