@@ -167,6 +167,15 @@ T0B_DEV uint32_t quantize8(const BlockScale<NV> &s, const float *v) {
   return NV && s.byte == 0 ? 0u : w;  // a scale of zero: no signs either
 }
 
+// One value of a block to a code, the same way.
+template <bool NV>
+T0B_DEV uint32_t quantize1(const BlockScale<NV> &s, float v) {
+  const float u = NV ? fmaf(v, s.hi, __fmul_rn(v, s.lo)) : v * s.hi;
+  uint32_t r;
+  asm("{\n .reg .b8 a;\n cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n mov.b32 %0, {a, a, a, a};\n}" : "=r"(r) : "f"(u), "f"(0.0f));
+  return NV && s.byte == 0 ? 0u : r & 15;
+}
+
 // ------------------------------------------------------------ quantisation
 // A lane takes 8 consecutive values of a row, a warp 256 (or, for short rows,
 // one scale tile's 64 or 128 of adjacent rows), each of the rows r, r + 32,
@@ -934,7 +943,7 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
 // itself (one launch, no 4-bit activations in memory).
 // Bound by its chain of latencies (launch, loads, MMA, exchange, stores): 1
 // token 512 x 512 3.0 us, 4096 x 4096 4.8 us (the pair kernel: 8.9); 19 tokens
-// gated 4096 x 1024 5.8 us (10.1); 333 x 1001 x 1000 5.4 us (9.9).
+// gated 4096 x 1024 5.2 us (10.1); 333 x 1001 x 1000 5.4 us (9.9).
 constexpr int SPLIT_THREADS = 256;
 constexpr int SPLIT_MAX_NS = 6, SPLIT_MAX_CLUSTER = 8;
 
@@ -956,26 +965,40 @@ struct SplitArgs {
   int xvec;
 };
 
-// One value per lane, 32 consecutive columns c0 .. c0 + 31 of row r (zeros
-// behind the matrix) to 4 bits.  Every lane of the warp calls it; c0 is a
-// multiple of 32.  Rows behind the matrix get zero scales.
+// One value per lane and row, 32 consecutive columns c0 .. c0 + 31 (zeros behind
+// the matrix) of `rows` <= 4 rows from r on, to 4 bits: largest magnitudes and
+// words of codes by shuffles, the rows side by side so that their latencies
+// overlap.  Every lane of the warp calls it; c0 is a multiple of 32.
 template <bool NV>
-T0B_DEV void quantize_lanes(const Fp4Mat &q, int r, int c0, float v) {
+T0B_DEV void quantize_lanes4(const Fp4Mat &q, int r, int rows, int c0, const float *v) {
   constexpr int BLK = NV ? 16 : 32;
   const int lane = threadIdx.x & 31, kt = (q.k + 4 * BLK - 1) / (4 * BLK);
-  float top = fabsf(v);
+  float top[4];
 #pragma unroll
-  for (int o = BLK / 2; o; o >>= 1) top = absmax(top, __shfl_xor_sync(0xFFFFFFFFu, top, o), 0.0f);
-  const BlockScale<NV> s(__float_as_uint(top), q);
-  // eight lanes' values to every eighth lane
-  float u[8];
+  for (int j = 0; j < 4; ++j) top[j] = fabsf(v[j]);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) u[j] = __shfl_sync(0xFFFFFFFFu, v, (lane & 24) + j);
-  const uint32_t w = quantize8<NV>(s, u);
+  for (int o = BLK / 2; o; o >>= 1)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) top[j] = absmax(top[j], __shfl_xor_sync(0xFFFFFFFFu, top[j], o), 0.0f);
+  uint32_t byte[4], w[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const BlockScale<NV> s(__float_as_uint(top[j]), q);
+    byte[j] = s.byte;
+    w[j] = quantize1<NV>(s, v[j]) << (4 * (lane & 7));
+  }
+#pragma unroll
+  for (int o = 1; o < 8; o *= 2)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[j] |= __shfl_xor_sync(0xFFFFFFFFu, w[j], o);
   const int b = (c0 + lane) / BLK;
-  if (lane % BLK == 0 && b < 4 * kt) q.scales[scale_at(r, b, kt)] = r < q.rows && b * BLK < q.k ? (uint8_t)s.byte : 0;
-  if (lane % 8 == 0 && r < q.rows && (c0 + lane) / 2 < (int)code_pitch(q.k))
-    *reinterpret_cast<uint32_t *>(q.codes + r * code_pitch(q.k) + (c0 + lane) / 2) = w;
+  const bool has_scale = lane % BLK == 0 && b < 4 * kt, has_codes = lane % 8 == 0 && (c0 + lane) / 2 < (int)code_pitch(q.k);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if (j >= rows) break;
+    if (has_scale) q.scales[scale_at(r + j, b, kt)] = b * BLK < q.k ? (uint8_t)byte[j] : 0;
+    if (has_codes) *reinterpret_cast<uint32_t *>(q.codes + (r + j) * code_pitch(q.k) + (c0 + lane) / 2) = w[j];
+  }
 }
 
 T0B_DEV void scale_cp(uint32_t taddr, uint64_t desc) {
@@ -1053,14 +1076,16 @@ T0B_DEV void quantize_slice(const SplitArgs &p, uint8_t *codes, uint8_t *scales,
         scales[(s * AT + lane / (4 * LB)) * 512 + (t & 31) * 16 + (t >> 5) * 4 + lane / LB % 4] =
             k_begin + s * 256 + lane * 8 < p.a.K ? (uint8_t)sc.byte : 0;
     };
-    if (i0 + (U - 1) * W < n) {  // without branches between them the pieces overlap
-#pragma unroll
-      for (int u = 0; u < U; ++u) piece(u);
-    } else {
-#pragma unroll
-      for (int u = 0; u < U - 1; ++u)
-        if (i0 + u * W < n) piece(u);
-    }
+    // without branches between them the pieces overlap
+    const int left = (n - i0 + W - 1) / W;
+    if (left >= 4)
+      piece(0), piece(1), piece(2), piece(3);
+    else if (left == 3)
+      piece(0), piece(1), piece(2);
+    else if (left == 2)
+      piece(0), piece(1);
+    else
+      piece(0);
   }
 }
 
@@ -1085,15 +1110,20 @@ T0B_DEV void split_results(const SplitArgs &p, uint8_t *slots, uint32_t tmem, in
   typename Plain<TY>::T *y = reinterpret_cast<typename Plain<TY>::T *>(p.a.y) + m0 * p.a.ld + n;
   const bool in = n < p.a.n;
   auto finish4 = [&](int t0, const float *g, const float *u) {  // tokens t0 .. t0 + 3 of the tile
+    float v[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      float v = fmaf(g[j], alpha, b0);
-      if constexpr (GLU) v = silu_mul(v, fmaf(u[j], alpha, b1));
-      if constexpr (OT >= 0) {
-        if (in && t0 + j < toks) y[(t0 + j) * p.a.ld] = Plain<TY>::put(v);
-      } else {
-        if (t0 + j < toks) quantize_lanes<NV>(p.a.q, m0 + t0 + j, n0 + 32 * (warp & 3), in ? v : 0.0f);
-      }
+      v[j] = fmaf(g[j], alpha, b0);
+      if constexpr (GLU) v[j] = silu_mul(v[j], fmaf(u[j], alpha, b1));
+    }
+    if constexpr (OT >= 0) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (in && t0 + j < toks) y[(t0 + j) * p.a.ld] = Plain<TY>::put(v[j]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = in ? v[j] : 0.0f;
+      quantize_lanes4<NV>(p.a.q, m0 + t0, min(4, toks - t0), n0 + 32 * (warp & 3), v);
     }
   };
   for (int t0 = 16 * half; t0 < toks && have; t0 += 32) {
