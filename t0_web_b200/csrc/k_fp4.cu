@@ -189,20 +189,33 @@ T0B_DEV uint32_t quantize1(const BlockScale<NV> &s, float v) {
 constexpr int QT_WARPS = 8;
 constexpr int QT_CHUNKS = 4;  // 65,536 x 1024 bf16: 39 us with 1, 35 with 2, 32 with 4 and 8
 
-// 8 values from x[k0 ..] as they lie in memory, zeros from k on; `vec`: rows
-// are 16-byte aligned.
+// 8 values from x[k0 ..] as they lie in memory, zeros from k on; `align`: the
+// rows start on this many bytes (16 or more, 8, 4, 2).
 template <int TY>
 struct Raw8 {
   using T = typename Plain<TY>::T;
   uint4 w[sizeof(T) / 2];
-  T0B_DEV void load(const T *x, int k0, int k, bool vec) {
-    if (vec && k0 + 8 <= k) {
+  T0B_DEV void load(const T *x, int k0, int k, int align) {
+    x += k0;
+    if (align >= 16 && k0 + 8 <= k) {
 #pragma unroll
-      for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = reinterpret_cast<const uint4 *>(x + k0)[i];
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = reinterpret_cast<const uint4 *>(x)[i];
+    } else if (align == 8 && k0 + 8 <= k) {
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
+        const uint2 a = reinterpret_cast<const uint2 *>(x)[2 * i], b = reinterpret_cast<const uint2 *>(x)[2 * i + 1];
+        w[i] = make_uint4(a.x, a.y, b.x, b.y);
+      }
+    } else if (align == 4 && k0 + 8 <= k) {
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
+        const uint32_t *p = reinterpret_cast<const uint32_t *>(x) + 4 * i;
+        w[i] = make_uint4(p[0], p[1], p[2], p[3]);
+      }
     } else {
       T e[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) e[i] = k0 + i < k ? x[k0 + i] : Plain<TY>::put(0.0f);
+      for (int i = 0; i < 8; ++i) e[i] = k0 + i < k ? x[i] : Plain<TY>::put(0.0f);
 #pragma unroll
       for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = reinterpret_cast<const uint4 *>(e)[i];
     }
@@ -210,6 +223,27 @@ struct Raw8 {
   T0B_DEV void zero() {
 #pragma unroll
     for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = make_uint4(0, 0, 0, 0);
+  }
+  // The same for the 256 values of a warp, x[c0 ..], of f32 rows that are not
+  // aligned: the lanes load neighbouring values, and turn() hands each lane
+  // its 8 through shared memory (256 values of the warp's own).  65,536 x 1001
+  // 55 us, 71 us with 8 loads of 4 bytes a lane.  (For 16-bit rows the turn
+  // costs more than it saves: 67 to 89 us against 59.)
+  T0B_DEV void load_turned(const T *x, int c0, int k) {
+    const int lane = threadIdx.x & 31, n = k - c0;
+    uint32_t *word = reinterpret_cast<uint32_t *>(w);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) word[i] = lane + 32 * i < n ? __float_as_uint(x[c0 + lane + 32 * i]) : 0u;
+  }
+  T0B_DEV void turn(uint32_t *sm) {
+    const int lane = threadIdx.x & 31;
+    const uint32_t *word = reinterpret_cast<const uint32_t *>(w);
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sm[lane + 32 * i] = word[i];
+    __syncwarp();
+    w[0] = reinterpret_cast<const uint4 *>(sm)[2 * lane];
+    w[1] = reinterpret_cast<const uint4 *>(sm)[2 * lane + 1];
   }
   T0B_DEV void get(float *v) const {
     const T *e = reinterpret_cast<const T *>(w);
@@ -221,9 +255,10 @@ struct Raw8 {
 // LPR: lanes along a row, 8 (one NV scale tile), 16 or 32.
 // A warp goes through `chunks` such pieces along its rows and fetches the next
 // one before it works on the present one.
-template <int TY, bool NV, int LPR>
+// TURN: f32 rows that are not aligned (LPR 32), see Raw8::load_turned.
+template <int TY, bool NV, int LPR, bool TURN>
 __global__ void __launch_bounds__(32 * QT_WARPS)
-    fp4_quantize_kernel(const typename Plain<TY>::T *x, int64_t ldx, Fp4Mat q, bool vec, int chunks) {
+    fp4_quantize_kernel(const typename Plain<TY>::T *x, int64_t ldx, Fp4Mat q, int align, int chunks) {
   constexpr int BLK = NV ? 16 : 32, LB = BLK / 8;  // lanes of a block
   constexpr int RPW = 32 / LPR;                    // adjacent rows of a warp
   const int kt = (q.k + 4 * BLK - 1) / (4 * BLK);
@@ -239,16 +274,21 @@ __global__ void __launch_bounds__(32 * QT_WARPS)
   uint8_t *scales = q.scales + ((size_t)group * kt + t0) * 512 + (r & 31) * 16 + 4 * b;
   const uint32_t sel1 = b & 1 ? 0x3715 : 0x6240, sel2 = b & 2 ? 0x3276 : 0x5410;
   const bool writes_scales = lane % LB == 0 && group < (q.rows + 127) / 128;
+  __shared__ __align__(16) uint32_t turned[TURN ? QT_WARPS : 1][TURN ? 256 : 4];
   pdl_wait();
   pdl_launch_dependents();
   Raw8<TY> next[4];
   auto fetch = [&](int k) {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      if (i < live)
-        next[i].load(row + 32 * i * ldx, k, q.k, vec);
-      else
+      if (i >= live) {
         next[i].zero();
+      } else {
+        if constexpr (TURN)
+          next[i].load_turned(row + 32 * i * ldx, k - 8 * lane, q.k);
+        else
+          next[i].load(row + 32 * i * ldx, k, q.k, align);
+      }
   };
   fetch(k0);
   for (int c = 0; c < chunks; ++c) {
@@ -261,6 +301,7 @@ __global__ void __launch_bounds__(32 * QT_WARPS)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       float v[8];
+      if constexpr (TURN) raw[i].turn(turned[threadIdx.x >> 5]);
       raw[i].get(v);
       float top = absmax_of<8>(v);
 #pragma unroll
@@ -962,7 +1003,7 @@ struct SplitArgs {
   int x_type;
   int64_t ldx;
   Fp4Mat xq;                // its scales' constants
-  int xvec;
+  int xalign;               // bytes its rows start on
 };
 
 // One value per lane and row, 32 consecutive columns c0 .. c0 + 31 (zeros behind
@@ -1052,7 +1093,7 @@ T0B_DEV void quantize_slice(const SplitArgs &p, uint8_t *codes, uint8_t *scales,
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int i = i0 + u * W, t = token(i);
-      if (i < n) next[u].load(x + (int64_t)(m0 + t) * p.ldx, k_begin + (i - t * stages) * 256 + lane * 8, p.a.K, p.xvec);
+      if (i < n) next[u].load(x + (int64_t)(m0 + t) * p.ldx, k_begin + (i - t * stages) * 256 + lane * 8, p.a.K, p.xalign);
     }
   };
   fetch(warp);
@@ -1423,7 +1464,12 @@ int max_pairs(const void *kfn, const cudaLaunchConfig_t &cfg) {
   return n;
 }
 
-bool rows_aligned(const void *p, int64_t ld, int type) { return ((uintptr_t)p | (uint64_t)ld * (type == TY_F32 ? 4 : 2)) % 16 == 0; }
+// The largest power of two up to 32 that the rows' addresses are multiples of.
+int rows_start(const void *p, int64_t ld, int type) {
+  const uint64_t a = (uintptr_t)p | (uint64_t)ld * (type == TY_F32 ? 4 : 2) | 32;
+  return (int)(a & (~a + 1));
+}
+bool rows_aligned(const void *p, int64_t ld, int type) { return rows_start(p, ld, type) >= 16; }
 
 int sm_count() {
   int dev = 0, n = 0;
@@ -1490,7 +1536,7 @@ cudaError_t launch_split(const Fp4Mat &w, const Fp4Mat &xm, const void *x, int x
   p.rot = GLU && a.up_row % 128;
   p.early = early;
   p.x = x, p.x_type = x_type, p.ldx = ldx, p.xq = xm;
-  p.xvec = FUSED && rows_aligned(x, ldx, x_type);
+  p.xalign = FUSED ? rows_start(x, ldx, x_type) : 0;
   p.stage = split_stage<NV, GLU, FUSED>(q.NT);
   const uint32_t fixed = (FUSED ? (uint32_t)q.SL * (q.NT * 128 + SC) : 0) +
                          (q.CS > 1 ? (uint32_t)(((q.NT + q.CS - 1) / q.CS + 3) / 4 * q.CS) * H * 2048 : 0) + 512 + 1024;
@@ -1597,8 +1643,7 @@ template <int TY, bool NV, bool QUANT>
 cudaError_t convert(const void *x, int64_t ld, const Fp4Mat &q, cudaStream_t st) {
   using T = typename Plain<TY>::T;
   constexpr int TILE = NV ? 8 : 16;
-  // expansion writes 32 bytes of f32 at once
-  const bool vec = QUANT || TY != TY_F32 ? rows_aligned(x, ld, TY) : ((uintptr_t)x | (uint64_t)ld * 4) % 32 == 0;
+  const int align = rows_start(x, ld, TY);
   const int lpr = q.k <= 8 * TILE ? TILE : q.k <= 128 ? 16 : 32;
   const int row_warps = (q.rows + 127) / 128 * lpr;  // of 32 / lpr rows, 32 rows a group
   const int width = QUANT ? (q.k + 8 * TILE - 1) / (8 * TILE) * (8 * TILE) : q.k;  // whole scale tiles
@@ -1607,13 +1652,17 @@ cudaError_t convert(const void *x, int64_t ld, const Fp4Mat &q, cudaStream_t st)
     // pieces of a row one after the other in a warp, as long as two waves of CTAs remain
     int chunks = 1;
     while (chunks < QT_CHUNKS && grid.y > 1 && (int64_t)grid.x * grid.y > 2 * 4 * sm_count()) chunks *= 2, grid.y = (grid.y + 1) / 2;
-    auto k = lpr == TILE ? fp4_quantize_kernel<TY, NV, TILE> : lpr == 16 ? fp4_quantize_kernel<TY, NV, 16> : fp4_quantize_kernel<TY, NV, 32>;
-    return launch(k, grid, 32 * QT_WARPS, st, (const T *)x, ld, q, vec, chunks);
+    auto k = lpr == TILE ? fp4_quantize_kernel<TY, NV, TILE, false>
+             : lpr == 16 ? fp4_quantize_kernel<TY, NV, 16, false>
+             : TY != TY_F32 || align >= 8 ? fp4_quantize_kernel<TY, NV, 32, false>
+                                          : fp4_quantize_kernel<TY, NV, 32, TY == TY_F32>;
+    return launch(k, grid, 32 * QT_WARPS, st, (const T *)x, ld, q, align, chunks);
   } else {
     auto k = lpr == TILE ? fp4_dequantize_kernel<TY, NV, TILE>
              : lpr == 16 ? fp4_dequantize_kernel<TY, NV, 16>
                          : fp4_dequantize_kernel<TY, NV, 32>;
-    return launch(k, grid, 32 * QT_WARPS, st, q, (T *)x, ld, vec);
+    // 8 values at once: 32 bytes of f32, 16 of the others
+    return launch(k, grid, 32 * QT_WARPS, st, q, (T *)x, ld, align >= (TY == TY_F32 ? 32 : 16));
   }
 }
 template <bool NV, bool QUANT>
