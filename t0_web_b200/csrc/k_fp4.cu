@@ -627,10 +627,22 @@ T0B_DEV void store_quant32(const Fp4Mat &q, int r, int c0, float *v) {
 }
 
 // 32 rows x 64 bytes of the result, one row per lane, columns c0 .. : through
-// the warp's staging buffer (64-byte swizzle) and out by a TMA store.
+// the warp's staging buffer (64-byte swizzle) and out by a TMA store.  A TMA
+// store ends a row on a 16-byte boundary, not at the tensor's last column: the
+// 64 bytes that hold the end of rows of another width are written value by
+// value, as nothing behind the last column may be touched.
 template <int TY>
 T0B_DEV void store_rows(const Fp4Args &p, const void *tm_y, uint8_t *stg, int row0, int c0, const float *v) {
   using T = typename Plain<TY>::T;
+  constexpr int W = 64 / sizeof(T);
+  if (c0 + W > p.n && p.n % (16 / (int)sizeof(T))) {
+    const int row = row0 + (threadIdx.x & 31);
+    T *y = reinterpret_cast<T *>(p.y) + row * p.ld + c0;
+#pragma unroll
+    for (int j = 0; j < W; ++j)
+      if (row < p.M && c0 + j < p.n) y[j] = Plain<TY>::put(v[j]);
+    return;
+  }
   const int lane = threadIdx.x & 31;
   if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
   __syncwarp();  // the buffer has been read
