@@ -142,7 +142,7 @@ struct BlockScale {
       const float a = __uint_as_float(amax);
       byte = e4m3_of(fmaf(a, q.r6_hi, a * q.r6_lo));  // a / (6 tensor_scale), the same way
       if (amax >= 0x7F800000u) byte = 127u;
-      const float d = e4m3_value(byte) * q.ts;
+      const float d = e4m3_value(min(byte, 126u)) * q.ts;  // finite: zeros stay zeros in a block of scale NaN too
       float r;
       asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
       hi = byte ? __uint_as_float(__float_as_uint(r) - 4u) : 0.0f;  // below 1 / d

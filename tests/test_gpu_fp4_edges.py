@@ -8,9 +8,51 @@ import torch
 
 import fp4_oracle as O
 from t0_web_b200 import fp4
-from test_gpu_fp4 import DEV, DT, FMT, check_close, mat_from, out_bound, rnd, sum_bound
+from test_gpu_fp4 import DEV, DT, FMT, check_close, empty, mat_from, out_bound, rnd, sum_bound
 
 pytestmark = pytest.mark.gpu
+
+
+# ---------------------------------------------------- zeros behind the matrix
+def check_padding(m):
+    """Codes behind k and scales of blocks and rows behind the matrix are zero."""
+    kp = -(-m.k // 32) * 32
+    code = O.unpack(m.codes.cpu().numpy(), m.scales.cpu().numpy(), m.rows, kp, m.format)[1]
+    assert not code[:, m.k:].any()
+    nb = -(-m.k // O.BLOCK[m.format])
+    s = m.scales.cpu().numpy().reshape(-(-m.rows // 128), -(-nb // 4), 32, 4, 4)
+    s = s.transpose(0, 3, 2, 1, 4).reshape(-(-m.rows // 128) * 128, -(-nb // 4) * 4)
+    assert not s[m.rows:].any() and not s[:, nb:].any()
+
+
+@pytest.mark.parametrize("fmt", FMT)
+@pytest.mark.parametrize("ty", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows,k,pad", [(3, 15, 1), (5, 17, 3), (200, 33, 0), (129, 100, 4), (33, 1001, 0), (140, 1001, 7), (2, 200, 8)])
+def test_codes_behind_k_of_blocks_with_nan(engine, fmt, ty, rows, k, pad):
+    x = torch.from_numpy(rnd(k, rows, k + pad)).to(DT[ty])[:, :k].to(DEV)
+    buf = torch.zeros((rows, k + pad), dtype=DT[ty], device=DEV)
+    x = buf[:, :k].copy_(x)
+    x[0, k - 1], x[rows - 1, k - 1] = float("nan"), float("-inf")
+    x[rows // 2, k - 1] = float("inf")
+    m = fp4.quantize(engine, x, empty(fmt, rows, k))
+    check_padding(m)
+    byte = O.unpack(m.codes.cpu().numpy(), m.scales.cpu().numpy(), rows, k, fmt)[0]
+    assert (byte[[0, rows // 2, rows - 1], -1] == (255 if fmt == "mx" else 127)).all()
+
+
+@pytest.mark.parametrize("fmt", FMT)
+@pytest.mark.parametrize("m", [1, 5, 40, 130, 700])  # few tokens, clusters, CTA pairs
+@pytest.mark.parametrize("f", [70, 257, 1001])
+def test_hidden_codes_behind_f_of_blocks_with_nan(engine, fmt, m, f):
+    k = 96
+    wv = rnd(f, 2 * f, k, dev=0.1)
+    wv[f - 1, 3] = np.nan  # the last gate row: the last hidden value of every token
+    w, _ = mat_from(wv, fmt)
+    x, _ = mat_from(rnd(m, m, k), fmt)
+    z = fp4.glu(engine, w, x, empty(fmt, m, f))
+    check_padding(z)
+    byte = O.unpack(z.codes.cpu().numpy(), z.scales.cpu().numpy(), m, f, fmt)[0]
+    assert (byte[:, -1] == (255 if fmt == "mx" else 127)).all() and (byte[:, :-1] < 127 + 128 * (fmt == "mx")).all()
 
 
 # ----------------------------------------------------------- aligned results
