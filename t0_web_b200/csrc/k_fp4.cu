@@ -419,12 +419,12 @@ __global__ void __launch_bounds__(32 * QT_WARPS) fp4_dequantize_kernel(Fp4Mat q,
 // ----------------------------------------------------------------- product
 // silu(g) * u.  1 / (1 + exp(-g)) with exp as 2^-t, t = g log2(e) carried to
 // twice the precision (the rounding error of t would otherwise grow with g);
-// beyond +-126 the sigmoid is 0 or 1 to the last bit, and the clamp keeps the
+// above 126 the sigmoid is 1 to the last bit, and the clamp keeps the
 // correction finite.
 constexpr float LOG2E = 1.44269504f, LOG2E_LO = 1.92596299e-8f, LN2 = 0.693147181f;
-T0B_DEV float ex2_neg(float t) {
+T0B_DEV float ex2_approx(float t) {
   float p;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p) : "f"(-t));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p) : "f"(t));
   return p;
 }
 T0B_DEV float rcp_approx(float x) {
@@ -432,13 +432,30 @@ T0B_DEV float rcp_approx(float x) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
-T0B_DEV float silu_mul(float g, float u) {
-  const float c = fminf(fmaxf(g, -126.0f), 126.0f);
+T0B_DEV float pow2(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
+// Below SILU_TAIL 1 / (1 + exp(-g)) is exp(g) to 2^-125, and soon no normal
+// number; its product with u may be one all the same.  exp(g) = 2^n 2^r, and
+// the powers of two are multiplied in one after the other, so that only the
+// result is rounded where it leaves the range.  From -208 on it is zero for
+// every u.
+constexpr float SILU_TAIL = 87.0f;
+T0B_DEV float silu_mul_tail(float g, float u) {
+  const float c = fmaxf(g, -208.0f) + (g - g);  // -infinity: NaN, as -infinity / (1 + exp(infinity))
+  const float n = rintf(c * LOG2E);             // -300 .. -125
+  const float r = fmaf(c, LOG2E_LO, fmaf(c, LOG2E, -n));
+  const float v = __fmul_rn(__fmul_rn(__fmul_rn(c, ex2_approx(r)), pow2(-120)), u);
+  const int e = (int)n + 120, half = e / 2;
+  return __fmul_rn(__fmul_rn(v, pow2(half)), pow2(e - half));
+}
+// For g >= -SILU_TAIL (or NaN).
+T0B_DEV float silu_mul_body(float g, float u) {
+  const float c = fminf(g, 126.0f);
   const float t = __fmul_rn(c, LOG2E);
   const float f = fmaf(fmaf(c, -LOG2E_LO, fmaf(c, -LOG2E, t)), LN2, 1.0f);
-  return __fmul_rn(__fmul_rn(g, rcp_approx(fmaf(ex2_neg(t), f, 1.0f))), u);
+  return __fmul_rn(__fmul_rn(g, rcp_approx(fmaf(ex2_approx(-t), f, 1.0f))), u);
 }
-// The same on pairs, for |g| below 2^20 (no clamp: the correction stays near 1
+T0B_DEV float silu_mul(float g, float u) { return g < -SILU_TAIL ? silu_mul_tail(g, u) : silu_mul_body(g, u); }
+// The body on pairs, for g below 2^20 (no clamp: the correction stays near 1
 // there), with the same results.
 T0B_DEV F2 silu_mul2(F2 g, F2 u) {
   const F2 t = mul2(g, F2(LOG2E, LOG2E));
@@ -446,7 +463,7 @@ T0B_DEV F2 silu_mul2(F2 g, F2 u) {
   const F2 f = fma2(e, F2(LN2, LN2), F2(1.0f, 1.0f));
   float t0, t1, d0, d1;
   t.get(t0, t1);
-  fma2(F2(ex2_neg(t0), ex2_neg(t1)), f, F2(1.0f, 1.0f)).get(d0, d1);
+  fma2(F2(ex2_approx(-t0), ex2_approx(-t1)), f, F2(1.0f, 1.0f)).get(d0, d1);
   return mul2(mul2(g, F2(rcp_approx(d0), rcp_approx(d1))), u);
 }
 
@@ -956,12 +973,25 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
           fma2(F2(u[j], u[j + 1]), alpha, F2(d.x, d.y)).get(u[j], u[j + 1]);
           fma2(F2(u[j + 2], u[j + 3]), alpha, F2(d.z, d.w)).get(u[j + 2], u[j + 3]);
         }
-        if (absmax_of<32>(g) < 1048576.0f) {
+        const float top = absmax_of<32>(g);
+        bool body = top <= SILU_TAIL;
+        if (!body) {
+          float low = 0.0f;
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) asm("min.f32 %0, %0, %1, %2;" : "+f"(low) : "f"(g[j]), "f"(g[j + 1]));
+          body = low >= -SILU_TAIL && top < 1048576.0f;
+        }
+        if (body) {
 #pragma unroll
           for (int j = 0; j < 32; j += 2) silu_mul2(F2(g[j], g[j + 1]), F2(u[j], u[j + 1])).get(v[j], v[j + 1]);
-        } else {
+        } else {  // rare: one value at a time, from local memory (unrolled, it cost the others 4 %)
+          float lg[32], lu[32];
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = silu_mul(g[j], u[j]);
+          for (int j = 0; j < 32; ++j) lg[j] = g[j], lu[j] = u[j];
+#pragma unroll 1
+          for (int j = 0; j < 32; ++j) lg[j] = silu_mul(lg[j], lu[j]);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = lg[j];
         }
         if constexpr (TY >= 0) {
 #pragma unroll
@@ -1165,9 +1195,21 @@ T0B_DEV void split_results(const SplitArgs &p, uint8_t *slots, uint32_t tmem, in
   auto finish4 = [&](int t0, const float *g, const float *u) {  // tokens t0 .. t0 + 3 of the tile
     float v[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      v[j] = fmaf(g[j], alpha, b0);
-      if constexpr (GLU) v[j] = silu_mul(v[j], fmaf(u[j], alpha, b1));
+    for (int j = 0; j < 4; ++j) v[j] = fmaf(g[j], alpha, b0);
+    if constexpr (GLU) {
+      float h[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) h[j] = fmaf(u[j], alpha, b1);
+      if (fminf(fminf(v[0], v[1]), fminf(v[2], v[3])) >= -SILU_TAIL) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = silu_mul_body(v[j], h[j]);
+      } else {
+        float lv[4] = {v[0], v[1], v[2], v[3]}, lh[4] = {h[0], h[1], h[2], h[3]};
+#pragma unroll 1
+        for (int j = 0; j < 4; ++j) lv[j] = silu_mul(lv[j], lh[j]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = lv[j];
+      }
     }
     if constexpr (OT >= 0) {
 #pragma unroll

@@ -55,6 +55,67 @@ def test_hidden_codes_behind_f_of_blocks_with_nan(engine, fmt, m, f):
     assert (byte[:, -1] == (255 if fmt == "mx" else 127)).all() and (byte[:, :-1] < 127 + 128 * (fmt == "mx")).all()
 
 
+# ---------------------------------------------------------------- the sigmoid
+@pytest.mark.parametrize("m", [3, 700])  # both product kernels
+@pytest.mark.parametrize("y_ty", ["f32", "bf16"])
+def test_glu_small_sigmoids_of_large_values(engine, m, y_ty):
+    """Gates down to -210 against up values to 3e38: products in range although the sigmoid alone is not.
+
+    The gates and up values are the biases (x = 0), exact in f32.  Bound: 8 units of 2^-24 for exp, quotient and products,
+    half a step of the output type, and two half steps of f32's smallest number where the result is subnormal."""
+    f = 640
+    rng = np.random.default_rng(7)
+    g = np.concatenate([np.linspace(-210, -80, f - 8), [-87, np.nextafter(np.float32(-87), np.float32(-100)), -87.3365, -87.34, -88.8, -103.9,
+                                                        -104.5, -120]]).astype(np.float32)
+    rng.shuffle(g)
+    u = (rng.choice([-1, 1], f) * 10.0 ** rng.uniform(0, 38.4, f)).astype(np.float32)
+    w, _ = mat_from(np.zeros((2 * f, 64)), "mx")
+    x, _ = mat_from(np.zeros((m, 64)), "mx")
+    z = torch.full((m, f), float("nan"), dtype=DT[y_ty], device=DEV)
+    fp4.glu(engine, w, x, z, torch.from_numpy(np.concatenate([g, u])).to(DEV))
+    fp4.sync(engine)
+    g, u = g.astype(np.float64), u.astype(np.float64)
+    ref = np.broadcast_to(g / (1 + np.exp(-g)) * u, (m, f))
+    check_close(z, ref, 8 * 2.0 ** -24 * np.abs(ref) + 2 * 2.0 ** -150 + out_bound(ref, y_ty) * (1 + 2.0 ** -10)
+                + (2.0 ** -134 if y_ty == "bf16" else 0))
+
+
+def test_glu_mixed_gates_on_both_kernels(engine):
+    """Ordinary gates beside large and small ones: the same bits from both product kernels, a group of 32 of one kind or mixed."""
+    f = 64 * 8
+    rng = np.random.default_rng(8)
+    g = rng.standard_normal((8, 64)) * 5
+    g[1], g[2], g[3] = rng.uniform(88, 3000, 64), rng.uniform(-150, -88, 64), rng.uniform(-200, 200, 64)
+    g[4, 7], g[5, 9], g[6, 11], g[7, 13] = 1e6, 1e30, -87.5, -1e30
+    g, u = g.reshape(-1).astype(np.float32), rng.standard_normal(f).astype(np.float32)
+    w, _ = mat_from(np.zeros((2 * f, 64)), "nv")
+    bias = torch.from_numpy(np.concatenate([g, u])).to(DEV)
+    got = []
+    for m in (3, 700):
+        x, _ = mat_from(np.zeros((m, 64)), "nv")
+        got.append(fp4.glu(engine, w, x, torch.full((m, f), float("nan"), device=DEV), bias))
+    fp4.sync(engine)
+    assert torch.equal(got[1], got[0][:1].expand(700, f)) and torch.equal(got[0], got[0][:1].expand(3, f))
+    g, u = g.astype(np.float64), u.astype(np.float64)
+    with np.errstate(over="ignore"):
+        ref = g / (1 + np.exp(-g)) * u
+    check_close(got[0][:1], ref[None], 8 * 2.0 ** -24 * np.abs(ref[None]) + 2 * 2.0 ** -150)
+
+
+def test_glu_infinite_gates_and_values(engine):
+    """silu(-inf) is NaN (-inf / inf) and silu(inf) infinite; a negative gate's finite factor leaves an infinity."""
+    f = 64
+    inf = float("inf")
+    g = torch.tensor([-inf, inf, -100.0, -1e38, float("nan"), 100.0, -50.0, 1e38], device=DEV).repeat(f // 8)
+    u = torch.tensor([1.0, 2.0, inf, 3e38, 1.0, -inf, inf, 1.0], device=DEV).repeat(f // 8)
+    w, _ = mat_from(np.zeros((2 * f, 64)), "mx")
+    for m in (3, 700):
+        x, _ = mat_from(np.zeros((m, 64)), "mx")
+        z = fp4.glu(engine, w, x, torch.empty((m, f), device=DEV), torch.cat([g, u])).cpu().numpy()
+        want = np.tile(np.array([np.nan, inf, -inf, 0, np.nan, -inf, -inf, 1e38], np.float32), f // 8)
+        assert np.array_equal(z, np.broadcast_to(want, z.shape), equal_nan=True)
+
+
 # ----------------------------------------------------------- aligned results
 @pytest.mark.parametrize("fmt", FMT)
 @pytest.mark.parametrize("m,f,k", [(300, 2048, 512), (700, 1000, 96), (1072, 2048, 512), (520, 1001, 70), (513, 384, 1024), (300, 260, 256),
