@@ -116,6 +116,10 @@ t0b_status guarded(F body) {
   }
 }
 
+// Clears the error word unless another error has been recorded since `seen`
+// was read: an error is cleared only by a call that reports it.
+__global__ void clear_error_kernel(int *err, int seen) { atomicCAS(err, seen, 0); }
+
 #define TRY(expr)                        \
   do {                                   \
     const t0b_status s_ = (expr);        \
@@ -270,7 +274,8 @@ extern "C" t0b_status t0b_fp4_sync(t0b_engine *e, void *stream) {
     TRY(cuda_status(fn, cudaMemcpyAsync(&herr, err, sizeof(int), cudaMemcpyDeviceToHost, st)));
     TRY(cuda_status(fn, cudaStreamSynchronize(st)));
     if (!herr) return T0B_OK;
-    TRY(cuda_status(fn, cudaMemsetAsync(err, 0, sizeof(int), st)));
+    clear_error_kernel<<<1, 1, 0, st>>>(err, herr);
+    TRY(cuda_status(fn, cudaGetLastError()));
     TRY(cuda_status(fn, cudaStreamSynchronize(st)));
     char what[80];
     snprintf(what, sizeof(what), "a kernel reported device error code %d", herr);

@@ -2,12 +2,17 @@
 
 Bounds of products and gated products: see test_gpu_fp4.py, whose helpers are used.
 """
+import ctypes as C
+import threading
+import time
+
 import numpy as np
 import pytest
 import torch
 
 import fp4_oracle as O
 from t0_web_b200 import fp4
+from t0_web_b200._lib import T0B_ERR_DEVICE, T0bError, lib
 from test_gpu_fp4 import DEV, DT, FMT, check_close, empty, mat_from, out_bound, rnd, sum_bound
 
 pytestmark = pytest.mark.gpu
@@ -53,6 +58,71 @@ def test_hidden_codes_behind_f_of_blocks_with_nan(engine, fmt, m, f):
     check_padding(z)
     byte = O.unpack(z.codes.cpu().numpy(), z.scales.cpu().numpy(), m, f, fmt)[0]
     assert (byte[:, -1] == (255 if fmt == "mx" else 127)).all() and (byte[:, :-1] < 127 + 128 * (fmt == "mx")).all()
+
+
+# ------------------------------------------------------------ error reporting
+class _Word:
+    """The engine's device error word of the 4-bit operators, as a tensor."""
+
+    def __init__(self, engine):
+        f = lib()["_Z18t0b_engine_fp4_errPK10t0b_engine"]
+        f.argtypes, f.restype = [C.c_void_p], C.c_void_p
+        self.__cuda_array_interface__ = dict(shape=(1,), typestr="<i4", data=(f(engine.handle), False), version=2)
+
+
+def error_word(engine):
+    return torch.as_tensor(_Word(engine), device=DEV)
+
+
+def test_error_of_a_kernel_is_reported_once(engine):
+    word = error_word(engine)
+    assert int(word) == 0
+    outcome = torch.zeros(1, dtype=torch.int32, device=DEV)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    wait = lib()["_Z32t0b_launch_bounded_wait_selftestPiS_P11CUstream_st"]
+    wait.argtypes = [C.c_void_p] * 3
+    assert wait(word.data_ptr(), outcome.data_ptr(), side.cuda_stream) == 0
+    with pytest.raises(T0bError) as e:
+        fp4.sync(engine, side.cuda_stream)
+    assert e.value.status == T0B_ERR_DEVICE and "error code 1" in str(e.value)
+    assert int(outcome) == 2
+    fp4.sync(engine, side.cuda_stream)
+    fp4.sync(engine)
+
+
+def test_errors_during_a_sync_are_not_lost(engine):
+    """An error recorded while another thread reads and clears the word is reported by that call or by the next."""
+    word = error_word(engine)
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    lost = []
+    for i in range(400):
+        said = []
+
+        def sync():
+            try:
+                fp4.sync(engine, a.cuda_stream)
+            except T0bError as e:
+                said.append(str(e))
+
+        with torch.cuda.stream(a):
+            word.fill_(1)
+        a.synchronize()
+        t = threading.Thread(target=sync)
+        t.start()
+        end = time.perf_counter() + (i % 100) * 2e-6
+        while time.perf_counter() < end:
+            pass
+        with torch.cuda.stream(b):
+            word.fill_(2)
+        b.synchronize()
+        t.join()
+        sync()
+        if not any("error code 2" in s for s in said):
+            lost.append(i)
+    word.zero_()
+    torch.cuda.synchronize()
+    assert not lost, f"{len(lost)} of 400"
 
 
 # ---------------------------------------------------------------- the sigmoid
