@@ -196,7 +196,16 @@ extern "C" t0b_status t0b_engine_create(int device, t0b_engine **out) {
                                          std::to_string(prop.major) + std::to_string(prop.minor));
   auto *e = new t0b_engine();
   e->device = device;
-  if (cudaMalloc(&e->d_err, 2 * sizeof(int)) != cudaSuccess || cudaMemset(e->d_err, 0, 2 * sizeof(int)) != cudaSuccess) {
+  // The error words are cleared on a stream of their own and before the engine
+  // is handed out: a clear on the default stream would wait behind its work
+  // and not come before what non-blocking streams read or record.
+  cudaStream_t st = nullptr;
+  bool ok = cudaMalloc(&e->d_err, 2 * sizeof(int)) == cudaSuccess &&
+            cudaStreamCreateWithFlags(&st, cudaStreamNonBlocking) == cudaSuccess;
+  ok = ok && cudaMemsetAsync(e->d_err, 0, 2 * sizeof(int), st) == cudaSuccess && cudaStreamSynchronize(st) == cudaSuccess;
+  if (st) cudaStreamDestroy(st);
+  if (!ok) {
+    if (e->d_err) cudaFree(e->d_err);
     delete e;
     return fail(T0B_ERR_OOM, "t0b_engine_create: device allocation failed");
   }

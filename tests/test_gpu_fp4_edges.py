@@ -11,7 +11,7 @@ import pytest
 import torch
 
 import fp4_oracle as O
-from t0_web_b200 import fp4
+from t0_web_b200 import fp4, t0_fast
 from t0_web_b200._lib import T0B_ERR_DEVICE, T0bError, lib
 from test_gpu_fp4 import DEV, DT, FMT, check_close, empty, mat_from, out_bound, rnd, sum_bound
 
@@ -123,6 +123,23 @@ def test_errors_during_a_sync_are_not_lost(engine):
     word.zero_()
     torch.cuda.synchronize()
     assert not lost, f"{len(lost)} of 400"
+
+
+def test_new_engine_has_no_errors_while_the_default_stream_is_busy():
+    e = t0_fast.Engine(0)
+    word = error_word(e)
+    at = word.data_ptr()
+    word.fill_(7)
+    torch.cuda.synchronize()
+    e.close()
+    side = torch.cuda.Stream()
+    torch.cuda._sleep(400_000_000)  # about 0.2 s on the legacy default stream
+    e = t0_fast.Engine(0)
+    fp4.sync(e, side.cuda_stream)  # a non-blocking stream: not ordered after the default one
+    if error_word(e).data_ptr() != at:
+        pytest.skip("the new engine's word lies elsewhere: nothing stale to see")
+    torch.cuda.synchronize()
+    e.close()
 
 
 # ---------------------------------------------------------------- the sigmoid
