@@ -273,11 +273,12 @@ t0b_status t0b_fp4_mlp(t0b_engine *e, const t0b_fp4 *w0, const t0b_fp4 *w2, int 
                        const t0b_fp4 *xq, const t0b_fp4 *zq, const float *b0_dev, const float *b2_dev, int y_type,
                        void *y_dev, int64_t ldy, void *stream);
 /* Wait for `stream` and report any kernel-side error of the engine's 4-bit
- * operators since the last call (not while `stream` is being captured).  An
- * error is the engine's, not the stream's: whichever call sees it first
- * reports and clears it (calls at the same time may all report it), and the
- * results of every stream that was at work are to be taken as unfinished.  One
- * that is recorded meanwhile is left for the next call. */
+ * operators since the last call (refused while `stream` is being captured,
+ * whose capture goes on).  An error is the engine's, not the stream's:
+ * whichever call sees it first reports and clears it (calls at the same time
+ * may all report it), and the results of every stream that was at work are to
+ * be taken as unfinished.  One that is recorded meanwhile is left for the next
+ * call. */
 t0b_status t0b_fp4_sync(t0b_engine *e, void *stream);
 
 /* ---- bounded-wait self-test (no reference counterpart; a diagnostic) ----

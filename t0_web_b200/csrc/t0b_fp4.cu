@@ -270,6 +270,10 @@ extern "C" t0b_status t0b_fp4_sync(t0b_engine *e, void *stream) {
     DeviceScope dev(t0b_engine_device(e));
     TRY(cuda_status(fn, dev.status));
     const cudaStream_t st = (cudaStream_t)stream;
+    // refused before anything is queued: a copy or wait would end the capture
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+    TRY(cuda_status(fn, cudaStreamIsCapturing(st, &capture)));
+    if (capture != cudaStreamCaptureStatusNone) return fail(T0B_ERR_INVALID, fn, "the stream is being captured");
     int *err = t0b_engine_fp4_err(e), herr = 0;
     TRY(cuda_status(fn, cudaMemcpyAsync(&herr, err, sizeof(int), cudaMemcpyDeviceToHost, st)));
     TRY(cuda_status(fn, cudaStreamSynchronize(st)));

@@ -142,6 +142,22 @@ def test_new_engine_has_no_errors_while_the_default_stream_is_busy():
     e.close()
 
 
+def test_sync_of_a_stream_under_capture_is_refused(engine):
+    w, _ = mat_from(rnd(1, 64, 96), "mx")
+    x, _ = mat_from(rnd(2, 5, 96), "mx")
+    y, want = torch.full((5, 64), float("nan"), device=DEV), torch.empty((5, 64), device=DEV)
+    fp4.gemm(engine, w, x, want)
+    torch.cuda.synchronize()
+    g, s = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(g, stream=s):
+        fp4.gemm(engine, w, x, y)
+        with pytest.raises(T0bError, match="captured"):
+            fp4.sync(engine)
+    g.replay()
+    fp4.sync(engine)
+    assert torch.equal(y, want)
+
+
 # ---------------------------------------------------------------- the sigmoid
 @pytest.mark.parametrize("m", [3, 700])  # both product kernels
 @pytest.mark.parametrize("y_ty", ["f32", "bf16"])
