@@ -15,6 +15,7 @@
 #include <mutex>
 
 #include "common.cuh"
+#include "fp4_plan.h"
 #include "t0b_internal.h"
 
 namespace {
@@ -1028,7 +1029,7 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
 // token 512 x 512 3.0 us, 4096 x 4096 4.8 us (the pair kernel: 8.9); 19 tokens
 // gated 4096 x 1024 5.2 us (10.1); 333 x 1001 x 1000 5.4 us (9.9).
 constexpr int SPLIT_THREADS = 256;
-constexpr int SPLIT_MAX_NS = 6, SPLIT_MAX_CLUSTER = 8;
+constexpr int SPLIT_MAX_NS = 6;
 
 struct SplitArgs {
   Fp4Args a;
@@ -1128,7 +1129,7 @@ T0B_DEV void quantize_slice(const SplitArgs &p, uint8_t *codes, uint8_t *scales,
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const auto *x = reinterpret_cast<const typename Plain<TY>::T *>(p.x);
   const int n = toks * stages;
-  const uint32_t inv = (65536u + (uint32_t)stages - 1) / (uint32_t)stages;  // i / stages for i < 4096, stages <= 8
+  const uint32_t inv = (65536u + (uint32_t)stages - 1) / (uint32_t)stages;  // i / stages for i < 4096, stages <= SPLIT_FUSED_MAX_SL
   auto token = [&](int i) { return (int)((uint32_t)i * inv >> 16); };
   Raw8<TY> next[U];
   auto fetch = [&](int i0) {
@@ -1531,58 +1532,13 @@ int sm_count() {
   return n;
 }
 
-// How a product is divided for the split kernel.
-struct SplitPlan {
-  int NT, CS, SL, rt;
-  int64_t ctas;
-  double us;  // estimate
-};
-// Tiles of 64 or 128 tokens where one does not hold them all (the scale columns
-// of a tile's first token have to be even: multiples of 64 tokens).
-SplitPlan split_plan(bool glu, int M, int n, int K, int most, int sms) {
-  SplitPlan q;
-  q.NT = M <= most ? (M + 7) / 8 * 8 : most;
-  q.rt = (n + 127) / 128;
-  const int64_t tiles = (int64_t)q.rt * ((M + q.NT - 1) / q.NT);
-  const int S = (K + 255) / 256;
-  // clusters have to fit the GPCs: of 8 CTAs not more than two thirds of the
-  // SMs can be used at once (1024 x 4096, 256 tokens in tiles of 128: 128 CTAs
-  // in clusters of 8 13.5 us, 96 in clusters of 4 for 384 tokens 8.4 us)
-  int cs = 1;
-  while (cs < SPLIT_MAX_CLUSTER && tiles * cs * 2 <= (cs == 4 ? sms * 2 / 3 : sms * 7 / 8) && S >= cs * 2) cs *= 2;
-  q.SL = (S + cs - 1) / cs;
-  q.CS = (S + q.SL - 1) / q.SL;
-  q.ctas = tiles * q.CS;
-  // microseconds, fitted to the measured times (within 15 % where either
-  // kernel is chosen): 512 x 512 3.3 (16 tokens), 4.6 (64); 8192 x 8192 9.8
-  // (16), 13.8 (128), 18.7 (256)
-  const double waves = (double)((q.ctas + sms - 1) / sms);
-  q.us = 2.6 + waves * ((glu ? 0.045 : 0.030) * q.NT + (glu ? 0.7 : 0.4) * q.SL);
-  return q;
-}
-// The same for the pair kernel: 256 tokens 512 x 512 4.8, 1024 x 4096 8.9,
-// 8192 x 8192 14.1; gated 512 x 512 5.5, 4096 x 4096 10.1.
-double pair_us(bool glu, int M, int n, int K, int sms) {
-  const int64_t tiles = (int64_t)((M + 255) / 256) * (glu ? (n + 127) / 128 : (n + 255) / 256);
-  return 3.9 + (double)((tiles + sms / 2 - 1) / (sms / 2)) * ((glu ? 1.1 : 0.5) + 0.31 * ((K + 255) / 256));
-}
-// The split kernel's plan if it is the faster one (CS 0: the pair kernel is).
-SplitPlan choose(bool glu, int M, int n, int K, int sms) {
-  SplitPlan q = split_plan(glu, M, n, K, 64, sms);
-  if (!glu && M > 64) {
-    const SplitPlan r = split_plan(glu, M, n, K, 128, sms);
-    if (r.us < q.us) q = r;
-  }
-  if (pair_us(glu, M, n, K, sms) <= q.us) q.CS = 0;
-  return q;
-}
-
 // x_type < 0: x is the 4-bit matrix xm; else plain, to be quantised as xm says.
 template <bool NV, bool GLU, bool FUSED>
 cudaError_t launch_split(const Fp4Mat &w, const Fp4Mat &xm, const void *x, int x_type, int64_t ldx, const Fp4Args &a, int out_type,
                          const SplitPlan &q, bool early, cudaStream_t st) {
   constexpr int AT = NV ? 4 : 2, H = GLU ? 2 : 1;
   constexpr uint32_t SC = AT * 512, LIMIT = 232448;
+  if (!split_plan_ok(q, GLU, FUSED, a.M, a.n, a.K)) return cudaErrorInvalidConfiguration;
   SplitArgs p{};
   p.a = a;
   p.NT = q.NT, p.CS = q.CS, p.SL = q.SL, p.rt = q.rt;
@@ -1788,7 +1744,7 @@ cudaError_t t0b_launch_fp4_linear(const Fp4Mat &w, int x_type, const void *x, in
     const Fp4Args a = product_args(w, xq, out, err);
     const SplitPlan q = choose(out.glu, a.M, a.n, a.K, sm_count());
     // its share of the activations stays in shared memory
-    if (q.CS && q.SL <= 8 && q.SL * 256 * a.M <= FUSED_MAX_VALUES)
+    if (q.CS && q.SL <= SPLIT_FUSED_MAX_SL && q.SL * 256 * a.M <= FUSED_MAX_VALUES)
       return split_dispatch<true>(w, xq, x, x_type, ldx, out, a, q, false, st);
   }
   const cudaError_t e = t0b_launch_fp4_quantize(x_type, x, ldx, xq, st);
