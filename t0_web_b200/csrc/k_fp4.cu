@@ -43,6 +43,15 @@ struct Plain<TY_BF16> {
   T0B_DEV static __nv_bfloat16 put(float v) { return __float2bfloat16_rn(v); }
 };
 
+// N values that are read or written as one word: aligned to it, wherever they lie.
+template <typename T, int N>
+struct alignas(N * sizeof(T) < 16 ? N * sizeof(T) : 16) Pack {
+  T v[N];
+};
+static_assert(alignof(Pack<float, 8>) >= alignof(uint4) && alignof(Pack<__half, 8>) >= alignof(uint4) &&
+                  alignof(Pack<__half, 2>) >= alignof(uint32_t) && alignof(Pack<__nv_bfloat16, 2>) >= alignof(uint32_t),
+              "packs are read as words");
+
 // ------------------------------------------------------------- the format
 T0B_DEV size_t code_pitch(int k) { return (size_t)((k + 31) / 32) * 16; }
 // byte of row r, block b in the scale tiles; kt = tiles along k
@@ -214,11 +223,11 @@ struct Raw8 {
         w[i] = make_uint4(p[0], p[1], p[2], p[3]);
       }
     } else {
-      T e[8];
+      Pack<T, 8> e;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) e[i] = k0 + i < k ? x[i] : Plain<TY>::put(0.0f);
+      for (int i = 0; i < 8; ++i) e.v[i] = k0 + i < k ? x[i] : Plain<TY>::put(0.0f);
 #pragma unroll
-      for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = reinterpret_cast<const uint4 *>(e)[i];
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = reinterpret_cast<const uint4 *>(&e)[i];
     }
   }
   T0B_DEV void zero() {
@@ -332,20 +341,20 @@ __global__ void __launch_bounds__(32 * QT_WARPS)
 template <int TY>
 T0B_DEV void store8(typename Plain<TY>::T *y, int k0, int k, bool vec, const float *v) {
   using T = typename Plain<TY>::T;
-  alignas(16) T t[8];
+  Pack<T, 8> t;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) t[i] = Plain<TY>::put(v[i]);
+  for (int i = 0; i < 8; ++i) t.v[i] = Plain<TY>::put(v[i]);
   if (vec && k0 + 8 <= k) {
     if constexpr (TY == TY_F32)
       asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(y + k0), "f"(v[0]), "f"(v[1]), "f"(v[2]),
                    "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
                    : "memory");
     else
-      *reinterpret_cast<uint4 *>(y + k0) = *reinterpret_cast<const uint4 *>(t);
+      *reinterpret_cast<uint4 *>(y + k0) = *reinterpret_cast<const uint4 *>(&t);
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      if (k0 + i < k) y[k0 + i] = t[i];
+      if (k0 + i < k) y[k0 + i] = t.v[i];
   }
 }
 // A warp's 256 values of a row that is not aligned, columns c0 .. of k, turned
@@ -371,8 +380,8 @@ T0B_DEV void store_unaligned(typename Plain<TY>::T *y, int c0, int k, typename P
       const int e = 2 * (lane + 32 * i) - odd;  // values e, e + 1 share a word
       if (e >= n || e > 255) break;
       if (e >= 0 && e + 1 < n) {
-        const T t[2] = {sm[e], sm[e + 1]};
-        *reinterpret_cast<uint32_t *>(y + e) = *reinterpret_cast<const uint32_t *>(t);
+        const Pack<T, 2> t{{sm[e], sm[e + 1]}};
+        *reinterpret_cast<uint32_t *>(y + e) = *reinterpret_cast<const uint32_t *>(&t);
       } else {
         y[e < 0 ? 0 : e] = sm[e < 0 ? 0 : e];
       }
@@ -667,10 +676,10 @@ T0B_DEV void store_rows(const Fp4Args &p, const void *tm_y, uint8_t *stg, int ro
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     constexpr int PER = 16 / sizeof(T);
-    alignas(16) T t[PER];
+    Pack<T, PER> t;
 #pragma unroll
-    for (int j = 0; j < PER; ++j) t[j] = Plain<TY>::put(v[i * PER + j]);
-    *reinterpret_cast<uint4 *>(stg + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4)) = *reinterpret_cast<const uint4 *>(t);
+    for (int j = 0; j < PER; ++j) t.v[j] = Plain<TY>::put(v[i * PER + j]);
+    *reinterpret_cast<uint4 *>(stg + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4)) = *reinterpret_cast<const uint4 *>(&t);
   }
   fence_proxy_async_smem();
   __syncwarp();
@@ -694,10 +703,10 @@ T0B_DEV void store_rows_unaligned(const Fp4Args &p, uint8_t *quarter, int q, int
   const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    alignas(16) T t[PER];
+    Pack<T, PER> t;
 #pragma unroll
-    for (int j = 0; j < PER; ++j) t[j] = Plain<TY>::put(v[i * PER + j]);
-    *reinterpret_cast<uint4 *>(quarter + lane * 256 + (((4 * h + i) ^ (lane & 15)) << 4)) = *reinterpret_cast<const uint4 *>(t);
+    for (int j = 0; j < PER; ++j) t.v[j] = Plain<TY>::put(v[i * PER + j]);
+    *reinterpret_cast<uint4 *>(quarter + lane * 256 + (((4 * h + i) ^ (lane & 15)) << 4)) = *reinterpret_cast<const uint4 *>(&t);
   }
   quarter_sync(q);
   const int first = c0 - W / 4 * h, n = p.n - first;
