@@ -733,6 +733,26 @@ T0B_DEV void store_rows_unaligned(const Fp4Args &p, uint8_t *quarter, int q, int
   quarter_sync(q);
 }
 
+// The scale tiles hold 128 rows from a multiple of 128 on; the up rows of a
+// gated tile start at F + f0, `off` rows into one.  Moves the scales of 128
+// rows from two row groups' tiles to their place in one (one warp, every lane
+// of which has waited for the tiles), ready for the async proxy.
+template <int AT>
+T0B_DEV void move_scales(uint8_t *to, const uint8_t *from, int off) {
+  const int lane = threadIdx.x & 31;
+  uint32_t *dst = reinterpret_cast<uint32_t *>(to);
+  const uint32_t *raw = reinterpret_cast<const uint32_t *>(from);
+#pragma unroll
+  for (int a = 0; a < AT; ++a)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int r = off + 32 * j + lane;
+      dst[a * 128 + lane * 4 + j] = raw[(r >> 7) * (AT * 128) + a * 128 + (r & 31) * 4 + ((r >> 5) & 3)];
+    }
+  fence_proxy_async_smem();
+  __syncwarp();
+}
+
 // TY: result type, or -1 for the 4-bit result of a gated product.
 template <bool NV, bool GLU, bool ROT, int TY>
 __global__ void __launch_bounds__(PAIR_THREADS, 1)
@@ -872,31 +892,16 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
       mbar_wait(mma_done, 0, p.err, T0B_DEVERR_WAIT_ACC, nullptr);
     } else if (ROT && warp == 2) {
       // ------------------------------------------------------------ up rows' scales (both CTAs)
-      // The scale tiles hold 128 rows from a multiple of 128 on; the up rows of
-      // a tile start at F + f0.  Moves them to their place in the tile.
       uint32_t g = 0;
       const int off = p.up_row & 127;
       bool ok = true;
       for (int tile = pair; tile < p.n_tiles && ok && !*abort_flag; tile += npairs) {
         for (int s = 0; s < S; ++s, ++g) {
           const uint32_t sl = g % NS;
-          bool got = true;
-          if (lane == 0) got = mbar_wait(&raw_full[sl], (g / NS) & 1, p.err, T0B_DEVERR_WAIT_W, abort_flag);
-          if (!__shfl_sync(0xFFFFFFFFu, got ? 1 : 0, 0)) {
-            ok = false;
-            break;
-          }
-          const uint32_t *raw = reinterpret_cast<const uint32_t *>(smem + sl * C::STAGE + C::OFF_RAW);
-          uint32_t *dst = reinterpret_cast<uint32_t *>(smem + sl * C::STAGE + C::OFF_SB + C::SC);
-#pragma unroll
-          for (int a = 0; a < AT; ++a)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const int r = off + 32 * j + lane;
-              dst[a * 128 + lane * 4 + j] = raw[(r >> 7) * (AT * 128) + a * 128 + (r & 31) * 4 + ((r >> 5) & 3)];
-            }
-          fence_proxy_async_smem();
-          __syncwarp();
+          ok = __all_sync(0xFFFFFFFFu, mbar_wait(&raw_full[sl], (g / NS) & 1, p.err, T0B_DEVERR_WAIT_W, abort_flag));
+          if (!ok) break;
+          uint8_t *st = smem + sl * C::STAGE;
+          move_scales<AT>(st + C::OFF_SB + C::SC, st + C::OFF_RAW, off);
           if (lane == 0) mbar_arrive_cluster(lead(&rot_full[sl]));
         }
       }
@@ -1433,20 +1438,9 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 1)
     const int off = p.a.up_row & 127;
     for (int i = 0; i < ns; ++i) {
       const int sl = i % NS;
-      bool got = true;
-      if (lane == 0) got = mbar_wait(&raw_full[sl], (i / NS) & 1, p.a.err, T0B_DEVERR_WAIT_W, abort_flag);
-      if (!__shfl_sync(0xFFFFFFFFu, got ? 1 : 0, 0)) break;
-      const uint32_t *raw = reinterpret_cast<const uint32_t *>(smem + sl * p.stage + OFF_RAW);
-      uint32_t *dst = reinterpret_cast<uint32_t *>(smem + sl * p.stage + OFF_WS + SC);
-#pragma unroll
-      for (int a = 0; a < AT; ++a)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int r = off + 32 * j + lane;
-          dst[a * 128 + lane * 4 + j] = raw[(r >> 7) * (AT * 128) + a * 128 + (r & 31) * 4 + ((r >> 5) & 3)];
-        }
-      fence_proxy_async_smem();
-      __syncwarp();
+      if (!__all_sync(0xFFFFFFFFu, mbar_wait(&raw_full[sl], (i / NS) & 1, p.a.err, T0B_DEVERR_WAIT_W, abort_flag))) break;
+      uint8_t *st = smem + sl * p.stage;
+      move_scales<AT>(st + OFF_WS + SC, st + OFF_RAW, off);
       if (lane == 0) mbar_arrive(&rot_full[sl]);
     }
   }
