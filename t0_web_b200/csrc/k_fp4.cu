@@ -844,6 +844,13 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
           }
         }
       }
+      // Copies in flight have landed before the shared memory is given up, also
+      // after a wait that ran out (CTA 0's barriers count both CTAs' copies, and
+      // both CTAs leave together).
+      for (uint32_t i = g > NS ? g - NS : 0; i < g; ++i) {
+        if (rank == 0) mbar_wait(&full[i % NS], (i / NS) & 1, p.err, T0B_DEVERR_WAIT_X, nullptr);
+        if (ROT) mbar_wait(&raw_full[i % NS], (i / NS) & 1, p.err, T0B_DEVERR_WAIT_W, nullptr);
+      }
     } else if (warp == 1 && rank == 0) {
       // ------------------------------------------------------------ MMA (CTA 0)
       constexpr uint32_t idesc = idesc_fp4<NV>(256, 256);
@@ -1397,10 +1404,16 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 1)
     __syncthreads();
   }
   if (loader) {
-    for (int i = first; i < ns; ++i) {
+    int i = first;
+    for (; i < ns; ++i) {
       if (!mbar_wait(&empty[i % NS], (i / NS - 1) & 1, p.a.err, T0B_DEVERR_WAIT_EMPTY, abort_flag)) break;
       load_w(i);
       if constexpr (!FUSED) load_x(i);
+    }
+    // copies in flight have landed before the shared memory is given up, also after a wait that ran out
+    for (int j = max(0, i - NS); j < i; ++j) {
+      mbar_wait(&full[j % NS], (j / NS) & 1, p.a.err, T0B_DEVERR_WAIT_X, nullptr);
+      if (GLU && p.rot) mbar_wait(&raw_full[j % NS], (j / NS) & 1, p.a.err, T0B_DEVERR_WAIT_W, nullptr);
     }
   } else if (warp == 1 && elect_one()) {
     // ------------------------------------------------------------ MMA
