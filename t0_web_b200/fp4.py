@@ -30,12 +30,17 @@ BLOCK = {"mx": 32, "nv": 16}
 _TYPES = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
 
 
+def _shape32(rows: int, k: int):
+    """The shape as the C calls take it; ctypes would cut larger numbers to 32 bits, so they become an invalid 0."""
+    return tuple(v if -(1 << 31) <= v < 1 << 31 else 0 for v in (rows, k))
+
+
 def code_bytes(rows: int, k: int) -> int:
-    return int(lib().t0b_fp4_code_bytes(rows, k))
+    return int(lib().t0b_fp4_code_bytes(*_shape32(rows, k)))
 
 
 def scale_bytes(fmt: str, rows: int, k: int) -> int:
-    return int(lib().t0b_fp4_scale_bytes(FORMATS[fmt], rows, k))
+    return int(lib().t0b_fp4_scale_bytes(FORMATS[fmt], *_shape32(rows, k)))
 
 
 class Fp4Matrix:
