@@ -276,3 +276,12 @@ def test_nothing_behind_the_last_column_is_written(engine, m, n):
             check_close(buf[:m, :n], r, b + out_bound(r, y_ty) * (1 + 2.0 ** -10))
             assert bool((buf[m:] == 77).all()) and bool((buf[:, n:] == 77).all())
     fp4.sync(engine)
+
+
+# ------------------------------------------------------------ threads, objects
+def test_matrices_cannot_be_changed_behind_their_pointers():
+    m = fp4.Fp4Matrix.empty("nv", 4, 64, DEV, 2.0 ** -6)
+    for name, v in (("codes", m.codes.clone()), ("scales", m.scales.clone()), ("tensor_scale", 0.5), ("rows", 3), ("k", 32), ("format", "mx")):
+        with pytest.raises(AttributeError):
+            setattr(m, name, v)
+    assert m.tensor_scale == 2.0 ** -6 and m._c.codes == m.codes.data_ptr()
