@@ -13,7 +13,7 @@ import torch
 import fp4_oracle as O
 from t0_web_b200 import fp4, t0_fast
 from t0_web_b200._lib import T0B_ERR_DEVICE, T0bError, lib
-from test_gpu_fp4 import DEV, DT, FMT, check_close, empty, mat_from, out_bound, rnd, sum_bound
+from test_gpu_fp4 import DEV, DT, FMT, TS, check_close, empty, mat_from, out_bound, rnd, sum_bound
 
 pytestmark = pytest.mark.gpu
 
@@ -279,9 +279,67 @@ def test_nothing_behind_the_last_column_is_written(engine, m, n):
 
 
 # ------------------------------------------------------------ threads, objects
+def test_threads_finish_their_work(engine):
+    k, n, rounds = 512, 700, 20
+    wq, _ = mat_from(rnd(1, n, k), "mx")
+    xs = [torch.from_numpy(rnd(i, 5 + 60 * i, k).astype(np.float32)).to(DEV) for i in range(4)]
+    want = [fp4.linear(engine, wq, x, empty("mx", len(x), k), torch.empty((len(x), n), device=DEV)).clone() for x in xs]
+    torch.cuda.synchronize()
+    bad, done = [], [0] * 4
+
+    def work(i):
+        try:
+            s = torch.cuda.Stream()
+            with torch.cuda.stream(s):
+                for _ in range(rounds):
+                    y = torch.empty((len(xs[i]), n), device=DEV)
+                    fp4.linear(engine, wq, xs[i], empty("mx", len(xs[i]), k), y)
+                    fp4.sync(engine)
+                    if not torch.equal(y, want[i]):
+                        bad.append(i)
+                    done[i] += 1
+        except Exception as e:  # noqa: BLE001  (an exception ends the thread only)
+            bad.append((i, repr(e)))
+
+    ts = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in ts:
+        t.start()
+    for t in ts:
+        t.join()
+    fp4.sync(engine)
+    assert not bad and done == [rounds] * 4
+
+
 def test_matrices_cannot_be_changed_behind_their_pointers():
     m = fp4.Fp4Matrix.empty("nv", 4, 64, DEV, 2.0 ** -6)
     for name, v in (("codes", m.codes.clone()), ("scales", m.scales.clone()), ("tensor_scale", 0.5), ("rows", 3), ("k", 32), ("format", "mx")):
         with pytest.raises(AttributeError):
             setattr(m, name, v)
     assert m.tensor_scale == 2.0 ** -6 and m._c.codes == m.codes.data_ptr()
+
+
+# ------------------------------------------------------------------ long sums
+@pytest.mark.parametrize("fmt", FMT)
+def test_longest_rows(engine, fmt):
+    """k = 2^20, the longest row there is: quantised, expanded, multiplied, gated."""
+    m, n, k = 9, 20, 1 << 20
+    xv = rnd(1, m, k).astype(np.float32)
+    xd = torch.from_numpy(xv).to(DEV)
+    xq = fp4.quantize(engine, xd, empty(fmt, m, k))
+    byte, code = O.quantize(xv, fmt, TS[fmt])
+    c, s = O.pack(byte, code, fmt)
+    assert np.array_equal(xq.codes.cpu().numpy(), c) and np.array_equal(xq.scales.cpu().numpy(), s)
+    x = O.values(byte, code, fmt, TS[fmt])
+    assert np.array_equal(fp4.dequantize(engine, xq, torch.empty_like(xd)).cpu().numpy(), x)
+    wq, w = mat_from(rnd(2, n, k, dev=2.0 ** -10), fmt)
+    ref, bound = x @ w.T, sum_bound(x, w)
+    y = fp4.gemm(engine, wq, xq, torch.empty((m, n), device=DEV))
+    check_close(y, ref, bound + 2.0 ** -24 * np.abs(ref))
+    y2 = fp4.linear(engine, wq, xd, empty(fmt, m, k), torch.empty((m, n), device=DEV))
+    assert torch.equal(y, y2)
+    z = fp4.glu(engine, wq, xq, torch.empty((m, n // 2), device=DEV))
+    fp4.sync(engine)
+    f = n // 2
+    e = bound + 2.0 ** -24 * np.abs(ref)
+    zr = O.glu(ref, f)
+    check_close(z, zr, 1.1 * e[:, :f] * (np.abs(ref[:, f:]) + e[:, f:]) + np.abs(ref[:, :f]) * e[:, f:] + 9 * 2.0 ** -24 * np.abs(zr))
