@@ -1194,6 +1194,11 @@ T0B_DEV void quantize_slice(const SplitArgs &p, uint8_t *codes, uint8_t *scales,
   }
 }
 
+// Four values with a gate below -SILU_TAIL among them: rare, and out of the way of the others.
+__device__ __noinline__ float4 silu_mul4(float4 g, float4 u) {
+  return make_float4(silu_mul(g.x, u.x), silu_mul(g.y, u.y), silu_mul(g.z, u.z), silu_mul(g.w, u.w));
+}
+
 // The results of a tile.  Warps 0 .. 3 and 4 .. 7 take alternate groups of 16
 // tokens; a thread has one weight row.  The slices' partial sums go to the CTA
 // that adds them as [source][four tokens][gate, up][row][token], 16 bytes a
@@ -1226,11 +1231,8 @@ T0B_DEV void split_results(const SplitArgs &p, uint8_t *slots, uint32_t tmem, in
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[j] = silu_mul_body(v[j], h[j]);
       } else {
-        float lv[4] = {v[0], v[1], v[2], v[3]}, lh[4] = {h[0], h[1], h[2], h[3]};
-#pragma unroll 1
-        for (int j = 0; j < 4; ++j) lv[j] = silu_mul(lv[j], lh[j]);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = lv[j];
+        const float4 r = silu_mul4(make_float4(v[0], v[1], v[2], v[3]), make_float4(h[0], h[1], h[2], h[3]));
+        v[0] = r.x, v[1] = r.y, v[2] = r.z, v[3] = r.w;
       }
     }
     if constexpr (OT >= 0) {
@@ -1293,6 +1295,11 @@ T0B_DEV void split_results(const SplitArgs &p, uint8_t *slots, uint32_t tmem, in
     if (m < (p.a.M + 127) / 128 * 128 && (int)threadIdx.x / 128 < TILES && t < kt)
       *reinterpret_cast<uint32_t *>(p.a.q.scales + scale_at(m, 4 * t, kt)) = 0;
   }
+}
+
+// Waits for the copies of the last of `issued` stages of a ring of NS.
+T0B_DEV void drain(uint64_t *full, int NS, int issued, int *err, int code) {
+  for (int i = max(0, issued - NS); i < issued; ++i) mbar_wait(&full[i % NS], (i / NS) & 1, err, code, nullptr);
 }
 
 template <bool NV, bool GLU, bool FUSED>
@@ -1403,17 +1410,12 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 1)
     fence_proxy_async_smem();
     __syncthreads();
   }
+  int issued = first;
   if (loader) {
-    int i = first;
-    for (; i < ns; ++i) {
-      if (!mbar_wait(&empty[i % NS], (i / NS - 1) & 1, p.a.err, T0B_DEVERR_WAIT_EMPTY, abort_flag)) break;
-      load_w(i);
-      if constexpr (!FUSED) load_x(i);
-    }
-    // copies in flight have landed before the shared memory is given up, also after a wait that ran out
-    for (int j = max(0, i - NS); j < i; ++j) {
-      mbar_wait(&full[j % NS], (j / NS) & 1, p.a.err, T0B_DEVERR_WAIT_X, nullptr);
-      if (GLU && p.rot) mbar_wait(&raw_full[j % NS], (j / NS) & 1, p.a.err, T0B_DEVERR_WAIT_W, nullptr);
+    for (; issued < ns; ++issued) {
+      if (!mbar_wait(&empty[issued % NS], (issued / NS - 1) & 1, p.a.err, T0B_DEVERR_WAIT_EMPTY, abort_flag)) break;
+      load_w(issued);
+      if constexpr (!FUSED) load_x(issued);
     }
   } else if (warp == 1 && elect_one()) {
     // ------------------------------------------------------------ MMA
@@ -1472,6 +1474,11 @@ __global__ void __launch_bounds__(SPLIT_THREADS, 1)
     split_results<NV, GLU, TY_F16>(p, slots, tmem, rank, n0, m0, toks, have);
   else
     split_results<NV, GLU, TY_BF16>(p, slots, tmem, rank, n0, m0, toks, have);
+  // after a wait that ran out: copies in flight land before the shared memory is given up
+  if (!have && loader) {
+    drain(full, NS, issued, p.a.err, T0B_DEVERR_WAIT_X);
+    if (GLU && p.rot) drain(raw_full, NS, issued, p.a.err, T0B_DEVERR_WAIT_W);
+  }
   __syncwarp();
   if (warp == 1) {
     tc_fence_after();
