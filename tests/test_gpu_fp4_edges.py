@@ -318,6 +318,24 @@ def test_matrices_cannot_be_changed_behind_their_pointers():
     assert m.tensor_scale == 2.0 ** -6 and m._c.codes == m.codes.data_ptr()
 
 
+# --------------------------------------------------------------- K slices
+@pytest.mark.parametrize("fmt", FMT)
+@pytest.mark.parametrize("k", [257, 513, 1281, 2305, 2600, 2817, 3329, 3585])  # clusters of 1 to 8, slices of unequal length
+@pytest.mark.parametrize("m", [1, 5, 40, 64])
+def test_every_cluster_size(engine, fmt, m, k):
+    n = 130
+    xq, x = mat_from(rnd(m + k, m, k), fmt)
+    wq, w = mat_from(rnd(k, 2 * n, k, dev=1.5 / np.sqrt(k)), fmt)
+    h, e = x @ w.T, sum_bound(x, w)
+    e = e + 2.0 ** -24 * np.abs(h)
+    y = fp4.gemm(engine, wq, xq, torch.full((m, 2 * n), float("nan"), device=DEV))
+    z = fp4.glu(engine, wq, xq, torch.full((m, n), float("nan"), device=DEV))
+    fp4.sync(engine)
+    check_close(y, h, e)
+    zr = O.glu(h, n)
+    check_close(z, zr, 1.1 * e[:, :n] * (np.abs(h[:, n:]) + e[:, n:]) + np.abs(h[:, :n]) * e[:, n:] + 9 * 2.0 ** -24 * np.abs(zr))
+
+
 # ------------------------------------------------------------------ long sums
 @pytest.mark.parametrize("fmt", FMT)
 def test_longest_rows(engine, fmt):
