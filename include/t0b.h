@@ -250,7 +250,9 @@ t0b_status t0b_fp4_quantize(t0b_engine *e, int x_type, const void *x_dev, int64_
  * elements. */
 t0b_status t0b_fp4_dequantize(t0b_engine *e, const t0b_fp4 *in, int y_type, void *y_dev, int64_t ldy, void *stream);
 /* y [x->rows, w->rows] = x . w^T (+ bias[w->rows], f32, may be NULL), of
- * y_type, row r at r * ldy elements; x and w of one format and k. */
+ * y_type, row r at r * ldy elements; x and w of one format and k, the product
+ * of their tensor scales a normal number.  Nothing of y behind column w->rows
+ * is touched. */
 t0b_status t0b_fp4_gemm(t0b_engine *e, const t0b_fp4 *w, const t0b_fp4 *x, const float *bias_dev, int y_type,
                         void *y_dev, int64_t ldy, void *stream);
 /* z = silu(x . gate^T + bg) * (x . up^T + bu), [x->rows, F] with w = gate rows

@@ -29,19 +29,23 @@ inline SplitPlan split_plan(bool glu, int M, int n, int K, int most, int sms) {
   q.SL = (S + cs - 1) / cs;
   q.CS = (S + q.SL - 1) / q.SL;
   q.ctas = tiles * q.CS;
-  // microseconds, fitted to the measured times (within 15 % where either
-  // kernel is chosen): 512 x 512 3.3 (16 tokens), 4.6 (64); 8192 x 8192 9.8
-  // (16), 13.8 (128), 18.7 (256)
+  // microseconds, fitted to the measured times of up to 512 tokens: 512 x 512
+  // 3.3 (16 tokens), 4.6 (64); 8192 x 8192 9.8 (16), 13.8 (128), 18.7 (256)
   const double waves = (double)((q.ctas + sms - 1) / sms);
   q.us = 2.6 + waves * ((glu ? 0.045 : 0.030) * q.NT + (glu ? 0.7 : 0.4) * q.SL);
   return q;
 }
+
 // The same for the pair kernel: 256 tokens 512 x 512 4.8, 1024 x 4096 8.9,
-// 8192 x 8192 14.1; gated 512 x 512 5.5, 4096 x 4096 10.1.
+// 8192 x 8192 14.1; gated 512 x 512 5.5, 4096 x 4096 10.1.  Too short for many
+// tokens (4096: 8192 x 64 9.6 for 14.5, 8192 x 8192 77 for 97), where the choice
+// is the same all the same; elsewhere the chosen kernel is within about 8 % of
+// the better one.
 inline double pair_us(bool glu, int M, int n, int K, int sms) {
   const int64_t tiles = (int64_t)((M + 255) / 256) * (glu ? (n + 127) / 128 : (n + 255) / 256);
   return 3.9 + (double)((tiles + sms / 2 - 1) / (sms / 2)) * ((glu ? 1.1 : 0.5) + 0.31 * ((K + 255) / 256));
 }
+
 // The split kernel's plan if it is the faster one (CS 0: the pair kernel is).
 inline SplitPlan choose(bool glu, int M, int n, int K, int sms) {
   SplitPlan q = split_plan(glu, M, n, K, 64, sms);

@@ -135,10 +135,12 @@ T0B_DEV float absmax_of(const float *v) {
 // largest magnitude (infinities and NaNs compare above every finite value).
 // Every rounding to 4 bits is decided as by the exact quotient.  MX: the
 // product with 1 / d is exact.  NV: d has four significant bits; 1 / d is held
-// as hi + lo to 2^-44, so u = fma(x, hi, x lo) is the quotient rounded to f32
-// (a quotient on a border is representable and comes out as itself, one that
-// is not differs from the border by at least 1.06 half ulps).  lo >= 0: the
-// sign of a zero and of an overflow stays.
+// as hi + lo to about 2^-41 (hi is below it by at most 5.5 units of 2^-23, and
+// one correction leaves the square of that), and u = fma(x, hi, x lo) is the
+// quotient so nearly that every border is decided rightly: a quotient on a
+// border is representable and comes out as itself, one that is not differs
+// from the border by at least 1.06 half ulps, a margin of some 2^-29.  lo >= 0:
+// the sign of a zero and of an overflow stays.
 template <bool NV>
 struct BlockScale {
   uint32_t byte;
@@ -593,10 +595,13 @@ struct Fp4Args {
 // tile's sums in registers and gives the columns back before it does anything
 // else; it works while the next tile is multiplied.
 // Bound by the tensor cores and, in a long run, by the power limit: 8192 x
-// 8192 x 8192 MX 170 us, NV 176 us (6.5 and 6.2 PFLOP/s); short K by the
-// epilogue: 65,536 x 1024 x 1024 to f32 56 us (268 MB written), gated and
-// quantised 32,768 x 4096 x 1024 MX 129 us, NV 143 us (two MUFU operations a
-// value).
+// 8192 x 8192 MX 170 to 177 us, NV 176 to 188 us in a graph of ten, by the box
+// (6.5 to 5.8 PFLOP/s; 192 and 199 us as single launches after a pause); short K by the
+// epilogue: 65,536 x 1024 x 1024 to f32 54 us (268 MB written), gated and
+// quantised 32,768 x 4096 x 1024 MX 131 to 134 us, NV 145 to 149 us.  There no
+// unit is full (XU 47 %, tensor pipe 43 %, issue 0.43 a cycle): the 16 epilogue
+// warps start on one barrier and go through loads, exp and reciprocal, and
+// quantisation in step, and the next tile waits for the one accumulator.
 // Measured and not kept: three accumulators of 128 columns in turn (equal,
 // NV 9 % slower: the MMA warp issues twice the MMAs); the scale copies by
 // another warp (8 % slower: one more hop a stage); token tiles fastest (equal).
@@ -693,8 +698,10 @@ T0B_DEV void store_rows(const Fp4Args &p, const void *tm_y, uint8_t *stg, int ro
 // a lane quarter bring their 64 bytes a row together in the quarter's 8 KB
 // (16-byte pieces swizzled by the row), and each writes 8 of the 32 rows, 256
 // bytes of a row at a time: the sectors at both ends are written in part, and
-// that is what unaligned rows cost.  32,768 x 4001 x 1024 to bf16 123 us, to
-// f32 187 us; with 64 bytes of a row at a time 214 and 309 us.
+// that is what unaligned rows cost.  32,768 x 4001 x 1024 to bf16 116 us, to
+// f32 189 us; with 64 bytes of a row at a time 214 and 309 us.  In aligned rows:
+// bf16 86 us (4008 values apart) to 70 us (4032 apart: 128 bytes), f32 97 to
+// 101 us.
 T0B_DEV void quarter_sync(int q) { asm volatile("bar.sync %0, 128;" ::"r"(2 + q) : "memory"); }
 template <int TY>
 T0B_DEV void store_rows_unaligned(const Fp4Args &p, uint8_t *quarter, int q, int h, int row0, int c0, const float *v) {

@@ -3,8 +3,8 @@
 An `Fp4Matrix` holds a matrix [rows, k] in 4 bits per value and one 8-bit scale
 per block of 32 values (format "mx", power-of-two scales) or 16 values ("nv",
 8-bit float scales times the matrix's own `tensor_scale`).  Operators take
-torch tensors on the engine's device: rows of any stride, unit stride along
-the columns, float32, float16 or bfloat16.
+torch tensors on the engine's device: float32, float16 or bfloat16, unit stride
+along the columns, rows any distance apart that does not make them overlap.
 
     engine = t0_fast.Engine(0)
     w = fp4.Fp4Matrix.empty("nv", n, k, "cuda:0", tensor_scale=2.0 ** -12)
@@ -15,7 +15,10 @@ the columns, float32, float16 or bfloat16.
 
 Every call queues work on `stream` (a cudaStream_t as an integer; by default
 torch's current stream of the engine's device) and returns; arguments that do
-not fit raise T0bError (or TypeError) before anything is queued.
+not fit raise T0bError (or TypeError) before anything is queued.  As with
+torch's own operators, a tensor that is used on another stream than its own
+has to outlive that use (`Tensor.record_stream`, or a reference kept until the
+stream has passed).
 """
 from __future__ import annotations
 
