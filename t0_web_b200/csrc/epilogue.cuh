@@ -51,6 +51,9 @@ struct Epi {
   const float *qn, *kn, *rope_t;
   float *ssq_qk;
   int p, E, H;
+  // the bias (and gnext) is a resident model's: no kernel writes it, so the
+  // small-M kernel may fetch it before the previous kernel has completed
+  bool bias_const;
 };
 
 // RoPE on 16 consecutive dims 16cg..16cg+15 (8 pairs) of a 64-dim head with

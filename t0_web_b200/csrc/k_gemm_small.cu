@@ -100,7 +100,10 @@ T0B_DEV void cluster_wait_acquire() { asm volatile("barrier.cluster.wait.acquire
 // Activations: the f16 planes ah / al [M][K], or, when x32 is given, the
 // f32 rows x32 [M][K], which each CTA splits into the planes of its K slice
 // in shared memory (standalone calls: no separate split kernel).
-template <int QT, int NT8>
+// EARLY: the bias and the next norm's gain are a resident model's and may be
+// fetched before the previous kernel has completed; a standalone call's bias
+// may come from that kernel.
+template <int QT, int NT8, bool EARLY>
 __global__ void __launch_bounds__(kThreads) gemm_q_small_kernel(const __half *__restrict__ ah,
                                                                 const __half *__restrict__ al,
                                                                 const float *__restrict__ x32, int M, int K,
@@ -132,9 +135,19 @@ __global__ void __launch_bounds__(kThreads) gemm_q_small_kernel(const __half *__
   const int f0 = blockIdx.x * 16;     // first hidden column (SWIGLU)
   if (cs > 1) cluster_arrive_relaxed();  // matched by the wait before the slot push
 
+  auto fetch_bias = [&] {
+    if (threadIdx.x < kRows) {
+      const int c = threadIdx.x;
+      if (epi.bias)
+        cp_async4(e_bias + c, epi.bias + (swiglu ? (c < 16 ? 0 : epi.F) + f0 + (c & 15) : n0 + c));
+      else
+        e_bias[c] = 0.0f;
+      if (resid) cp_async4(e_gain + c, epi.gnext + n0 + c);
+    }
+  };
   // 1. constant operands (may be fetched while the previous kernel is still
-  //    running): the raw weight blocks of the 32 rows for this K slice, the
-  //    bias and the next norm's gain
+  //    running): the raw weight blocks of the 32 rows for this K slice, EARLY
+  //    the bias and the next norm's gain
   {
     // warp w stages rows w, w + 4, ...; lane q its 16-byte granules q, q + 32, ...
     const int gpr = (int)(L.wpitch / 16);  // granules per row: 17 (Q8_0) / 9 (Q4_0) per 256 values
@@ -144,20 +157,14 @@ __global__ void __launch_bounds__(kThreads) gemm_q_small_kernel(const __half *__
       if (!T0B_CHECK(wrow < (swiglu ? 2 * epi.F : epi.N), err)) continue;
       for (int q = lane; q < gpr; q += 32) cp_async16(wst + r * L.wpitch + q * 16, src + q * 16);
     }
-    if (threadIdx.x < kRows) {
-      const int c = threadIdx.x;
-      if (epi.bias)
-        cp_async4(e_bias + c, epi.bias + (swiglu ? (c < 16 ? 0 : epi.F) + f0 + (c & 15) : n0 + c));
-      else
-        e_bias[c] = 0.0f;
-      if (resid) cp_async4(e_gain + c, epi.gnext + n0 + c);
-    }
+    if constexpr (EARLY) fetch_bias();
     cp_async_commit();
   }
-  // 2. operands written by earlier kernels: activations, residual rows and
-  //    RMSNorm partial sums
+  // 2. operands written by earlier kernels: activations, residual rows,
+  //    RMSNorm partial sums, and the bias of a standalone call
   pdl_wait();
   {
+    if constexpr (!EARLY) fetch_bias();
     if (x32) {
       // f32 activation rows (token) by warp, 16-byte granules by lane
       float *xs = reinterpret_cast<float *>(smem + L.xs_off);
@@ -380,7 +387,7 @@ cudaError_t launch_small_t(const __half *ah, const __half *al, const float *x32,
   constexpr int MT = 8 * NT8;
   const int cs = K / KS;
   const SmallLayout L = small_layout(QT, KS, MT, cs, epi.ssq_in ? epi.ssq_in_nt : 0, x32 != nullptr);
-  auto kfn = gemm_q_small_kernel<QT, NT8>;
+  auto kfn = epi.bias_const ? gemm_q_small_kernel<QT, NT8, true> : gemm_q_small_kernel<QT, NT8, false>;
   cudaError_t e = t0b_smem_limit((const void *)kfn, L.bytes);
   if (e != cudaSuccess) return e;
   const int gx = epi.kind == EPI_SWIGLU ? epi.F / 16 : epi.N / kRows;

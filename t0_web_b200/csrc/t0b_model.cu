@@ -573,6 +573,7 @@ void fold_records(t0b_model *m) {
 
 cudaError_t qgemm(t0b_model *m, const __half *ah, const __half *al, int M, int K, const uint8_t *W, int wrows,
                   int wshift, Epi &epi) {
+  epi.bias_const = true;
   // algorithmic work: 2 M N K flops; bytes = raw weight blocks + A (as f32) +
   // the f32 output (SWIGLU writes F columns; RESID also reads the residual)
   const double wbytes = (double)wrows * K / 32.0 * (m->qt == 8 ? 34.0 : 18.0);
