@@ -599,7 +599,7 @@ struct Fp4Args {
 // (6.5 to 5.8 PFLOP/s; 192 and 199 us as single launches after a pause); short K by the
 // epilogue: 65,536 x 1024 x 1024 to f32 54 us (268 MB written), gated and
 // quantised 32,768 x 4096 x 1024 MX 131 to 134 us, NV 145 to 149 us.  There no
-// unit is full (XU 47 %, tensor pipe 43 %, issue 0.43 a cycle): the 16 epilogue
+// unit is full (XU 47 %, tensor pipe 42 %, issue 0.44 a cycle): the 16 epilogue
 // warps start on one barrier and go through loads, exp and reciprocal, and
 // quantisation in step, and the next tile waits for the one accumulator.
 // Measured and not kept: three accumulators of 128 columns in turn (equal,
