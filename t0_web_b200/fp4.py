@@ -49,7 +49,7 @@ def scale_bytes(fmt: str, rows: int, k: int) -> int:
 class Fp4Matrix:
     """A 4-bit matrix over two uint8 tensors (layout: include/t0b.h), which it keeps alive.
 
-    Its attributes cannot be set anew: calls go by the pointers taken here.  (The tensors' contents may be written.)"""
+    What it holds cannot be set anew: calls go by the pointers taken here.  (The tensors' contents may be written.)"""
 
     def __init__(self, fmt: str, rows: int, k: int, codes: torch.Tensor, scales: torch.Tensor, tensor_scale: float = 1.0):
         if fmt not in FORMATS:
@@ -69,7 +69,7 @@ class Fp4Matrix:
         self._ref = C.byref(self._c)
 
     def __setattr__(self, name, value):
-        if "_ref" in self.__dict__:
+        if "_ref" in self.__dict__ and name in self.__dict__:
             raise AttributeError(f"Fp4Matrix: {name} cannot be set, make another matrix")
         object.__setattr__(self, name, value)
 

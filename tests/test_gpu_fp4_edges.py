@@ -316,6 +316,8 @@ def test_matrices_cannot_be_changed_behind_their_pointers():
         with pytest.raises(AttributeError):
             setattr(m, name, v)
     assert m.tensor_scale == 2.0 ** -6 and m._c.codes == m.codes.data_ptr()
+    m.label = "a user's own attribute"
+    assert m.label
 
 
 # --------------------------------------------------------------- K slices
