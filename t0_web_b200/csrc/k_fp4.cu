@@ -595,7 +595,7 @@ struct Fp4Args {
 // tile's sums in registers and gives the columns back before it does anything
 // else; it works while the next tile is multiplied.
 // Bound by the tensor cores and, in a long run, by the power limit: 8192 x
-// 8192 x 8192 MX 170 to 177 us, NV 176 to 188 us in a graph of ten, by the box
+// 8192 x 8192 MX 170 to 177 us, NV 176 to 188 us in a graph of ten, by the card
 // (6.5 to 5.8 PFLOP/s; 192 and 199 us as single launches after a pause); short K by the
 // epilogue: 65,536 x 1024 x 1024 to f32 54 us (268 MB written), gated and
 // quantised 32,768 x 4096 x 1024 MX 131 to 134 us, NV 145 to 149 us.  There no
